@@ -35,7 +35,8 @@ __device__ __forceinline__ IbSplit ib_split2(float a, float b) {
   r.l = ib_pk(ra - ib_lo(r.m), rb - ib_hi(r.m));
   return r;
 }
-// the same split on a float pair, the differences as packed fp32 (v_pk_add_f32): 9 VALU per pair
+// the same split on a float pair, written on two-element vectors (the library is built without packed
+// fp32 instructions, so each difference is two adds)
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 // (the empty asm keeps hipcc from re-deriving the low half by a second v_cvt_pk_bf16_f32 of the
 // first element alone: one VALU per stage)
