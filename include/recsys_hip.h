@@ -805,6 +805,43 @@ int rs_rank_metrics_i64(const int64_t* pred, int64_t U, int K, const int32_t* le
  * alias x. */
 int rs_l2_normalize_rows_f32(const float* x, int64_t n, int64_t D, float* out, rs_stream_t stream);
 
+/* ---- softmax cross entropy over a whole catalogue ---------------------------------------------
+ * The full-catalogue form of the retrieval loss (tfrs.tasks.Retrieval, src/models.py:116,137, whose
+ * vocabulary is the batch's own items). X [N][D] rows, W [V][D] items (D <= 256; both RS_DTYPE_F32 or
+ * both RS_DTYPE_BF16), labels [N] in [0, V) or ignore_index, scale c > 0, weights a [N] (nullable: 1):
+ *   s_nv = c <x_n, w_v>, lse_n = log sum_v exp s_nv, row_n = lse_n - s_n,label, loss = sum a_n row_n / Z,
+ * Z = 1, or with `mean` the sum of a over the labelled rows (no labelled row: loss 0). No logits are
+ * stored. An ignored row has row_loss 0, enters neither loss nor gradients (whatever its x holds) and
+ * has the lse of its finite entries; a label that is neither in range nor ignore_index makes its row
+ * loss, its dX row and the loss NaN and stays out of dW. row_loss, lse [N] and *loss are fp32.
+ * want: RS_CATALOG_DX / _DW: which gradients a backward will be asked for (0: the loss alone, about
+ * half the work). `keep` (rs_catalog_softmax_keep_bytes, same arguments) carries the forward's state to
+ * the backward and is only read there; the workspace may be reused after each call. X, W, keep,
+ * workspace, dX and dW are 16-byte aligned. The backward takes the same W and arguments, gscale =
+ * dL/dloss on the device (NULL: 1), and writes dX [N][D] and dW [V][D] (either may be NULL) in the inputs'
+ * type. Sums run in a fixed order: equal calls give equal bits. */
+enum { RS_DTYPE_F32 = 0, RS_DTYPE_BF16 = 1 };
+enum { RS_CATALOG_DX = 1, RS_CATALOG_DW = 2 };
+size_t rs_catalog_softmax_keep_bytes(int64_t N, int64_t V, int64_t D, int dtype, int want);
+size_t rs_catalog_softmax_workspace_bytes(int64_t N, int64_t V, int64_t D, int dtype, int want);
+int rs_catalog_softmax_fwd(const void* X, const void* W, const int64_t* labels, const float* weights, int64_t N,
+                           int64_t V, int64_t D, int dtype, float scale, int64_t ignore_index, int mean, int want,
+                           float* loss, float* row_loss, float* lse, void* keep, size_t keep_bytes, void* workspace,
+                           size_t workspace_bytes, rs_stream_t stream);
+int rs_catalog_softmax_bwd(const void* W, int64_t N, int64_t V, int64_t D, int dtype, float scale, int want,
+                           const float* gscale, const void* keep, size_t keep_bytes, void* dX, void* dW,
+                           void* workspace, size_t workspace_bytes, rs_stream_t stream);
+
+/* ---- dropout ------------------------------------------------------------------------------------
+ * keras.layers.Dropout (the reference's dropout_rate, src/config.py:21, src/models.py:16,22): y = x /
+ * (1 - rate) where element i's word is at least round(rate 2^32), else 0. Words: Philox4x32-10 with key =
+ * ticket[0] and counter (i / 4, ticket[1]), word i % 4; ticket is int64 [2] on the device. The backward is
+ * the same call on dy with the same ticket. x and y hold n elements of dtype; y may be x.
+ * rs_dropout_ticket copies state (int64 [2]: seed, step) to ticket and adds one to the step, on the
+ * device, so a captured step draws a new mask at each replay. */
+int rs_dropout(const void* x, int64_t n, int dtype, double rate, const int64_t* ticket, void* y, rs_stream_t stream);
+int rs_dropout_ticket(int64_t* state, int64_t* ticket, rs_stream_t stream);
+
 /* ---- input pipeline -------------------------------------------------------
  * Replaces ds.shuffle(50000) of make_ds (src/trainer.py:115-116): the epoch's element order under
  * tf.data's shuffle-buffer process (a buffer of buffer_size elements; each output is a uniformly

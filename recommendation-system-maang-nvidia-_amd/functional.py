@@ -2,8 +2,8 @@
 
 Every op here launches hand-written gfx950 kernels from librecsys_hip.so on the current
 PyTorch (HIP) stream; PyTorch only supplies device memory, streams and autograd plumbing.
-Inputs must be contiguous float32 (int64 for ids) tensors on a ROCm device; anything else
-raises — there is no CPU or eager fallback.
+Inputs must be contiguous float32 (int64 for ids) tensors on a ROCm device (the catalogue softmax
+and dropout also take bfloat16); anything else raises — there is no CPU or eager fallback.
 """
 from __future__ import annotations
 
@@ -1357,6 +1357,149 @@ def l2_normalize_rows(x: torch.Tensor, out: Optional[torch.Tensor] = None) -> to
 
 
 # --------------------------------------------------------------------------------------------
+# softmax cross entropy over a whole catalogue; dropout (fp32 or bf16 operands)
+# --------------------------------------------------------------------------------------------
+RS_DTYPES = {torch.float32: 0, torch.bfloat16: 1}   # include/recsys_hip.h RS_DTYPE_*
+RS_CATALOG_DX, RS_CATALOG_DW = 1, 2                  # include/recsys_hip.h
+CATALOG_MAX_WIDTH = 256
+REDUCTIONS = ("sum", "mean")
+
+
+def _dev_typed(t: torch.Tensor, name: str) -> torch.Tensor:
+    """_dev for the operators that take fp32 or bf16."""
+    if t.is_cuda and t.dtype not in RS_DTYPES:
+        raise TypeError(f"{name}: expected float32 or bfloat16, got {t.dtype}")
+    return _dev(t, name, t.dtype)
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """t, or a copy of it where its storage offset leaves it off a 16-byte boundary."""
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+class CatalogSoftmaxState:
+    """What catalog_softmax_fwd hands to catalog_softmax_bwd: the operands' images, the rows'
+    statistics and the unit gradient of X, in one buffer that the backward only reads."""
+    __slots__ = ("keep", "N", "V", "D", "dtype", "scale", "want")
+
+    def __init__(self, keep, N, V, D, dtype, scale, want):
+        self.keep, self.N, self.V, self.D, self.dtype, self.scale, self.want = keep, N, V, D, dtype, scale, want
+
+
+def _catalog_check(X, W, labels, weights, scale, reduction):
+    _dev_typed(X, "X"), _dev_typed(W, "W"), _dev(labels, "labels", torch.int64)
+    if X.dim() != 2 or W.dim() != 2 or X.shape[1] != W.shape[1]:
+        raise ValueError(f"catalog_softmax: X [N, D] and W [V, D] expected, got {tuple(X.shape)} and {tuple(W.shape)}")
+    if X.dtype != W.dtype:
+        raise TypeError(f"catalog_softmax: X is {X.dtype}, W is {W.dtype}")
+    if labels.shape != X.shape[:1]:
+        raise ValueError(f"catalog_softmax: labels must be [{X.shape[0]}], got {tuple(labels.shape)}")
+    if weights is not None and _dev(weights, "weights").shape != X.shape[:1]:
+        raise ValueError(f"catalog_softmax: weights must be [{X.shape[0]}], got {tuple(weights.shape)}")
+    if any(t is not None and t.device != X.device for t in (W, labels, weights)):
+        raise ValueError("catalog_softmax: X, W, labels and weights must be on one device")
+    if W.shape[0] < 1 or X.shape[1] < 1:
+        raise ValueError("catalog_softmax: an empty catalogue or width")
+    if X.shape[1] > CATALOG_MAX_WIDTH:
+        raise NotImplementedError(f"catalog_softmax: width {X.shape[1]} > {CATALOG_MAX_WIDTH}")
+    if not (0.0 < scale < float("inf")):
+        raise ValueError(f"catalog_softmax: scale must be positive and finite, got {scale!r}")
+    if reduction not in REDUCTIONS:
+        raise ValueError(f"catalog_softmax: reduction must be one of {REDUCTIONS}, got {reduction!r}")
+
+
+def catalog_softmax_fwd(X, W, labels, scale: float = 1.0, weights=None, ignore_index: int = -100,
+                        reduction: str = "sum", want_grad=True):
+    """Softmax cross entropy of rows X [N, D] over all V items W [V, D] (rs_catalog_softmax_fwd; both
+    float32 or both bfloat16, D <= 256), labels int64 [N] item rows or ignore_index, logits
+    scale * X W^T, optional float32 row weights [N]. Returns (loss fp32 0-dim, row_loss [N], lse [N],
+    state): loss = sum of weight * row_loss over the labelled rows, divided by the sum of their
+    weights for reduction "mean" (0 without a labelled row); state is for catalog_softmax_bwd.
+    want_grad: False (the loss alone, about half the work), True, or a pair (dX, dW) of bools.
+    A label outside [0, V) that is not ignore_index makes its row and the loss NaN."""
+    X, W = X.detach(), W.detach()
+    _catalog_check(X, W, labels, weights, scale, reduction)
+    want_x, want_w = want_grad if isinstance(want_grad, (tuple, list)) else (want_grad, want_grad)
+    want = (RS_CATALOG_DX if want_x else 0) | (RS_CATALOG_DW if want_w else 0)
+    X, W = _aligned(X), _aligned(W)
+    (N, D), V, dt = X.shape, W.shape[0], RS_DTYPES[X.dtype]
+    dev = X.device
+    with torch.cuda.device(dev):
+        keep = _ws(query("rs_catalog_softmax_keep_bytes", N, V, D, dt, want), dev)
+        ws = _ws(query("rs_catalog_softmax_workspace_bytes", N, V, D, dt, want), dev)
+        loss = torch.empty((), dtype=torch.float32, device=dev)
+        row = torch.empty((N,), dtype=torch.float32, device=dev)
+        lse = torch.empty((N,), dtype=torch.float32, device=dev)
+        call("rs_catalog_softmax_fwd", _p(X), _p(W), _p(labels), _p(weights), N, V, D, dt, float(scale),
+             int(ignore_index), int(reduction == "mean"), want, _p(loss), _p(row), _p(lse), _p(keep), keep.numel(),
+             _p(ws), ws.numel(), _stream())
+    return loss, row, lse, CatalogSoftmaxState(keep, N, V, D, X.dtype, float(scale), want)
+
+
+def catalog_softmax_bwd(W, state: CatalogSoftmaxState, g=None, dx: bool = True, dw: bool = True):
+    """Gradients of catalog_softmax_fwd's loss -> (dX or None, dW or None) in the inputs' type. W: the
+    forward's; g: dL/dloss (float32 0-dim on the device; None: 1). A forward's state may be used for
+    several backwards."""
+    W = W.detach()
+    _dev(W, "W", state.dtype)
+    if tuple(W.shape) != (state.V, state.D) or W.device != state.keep.device:
+        raise ValueError("catalog_softmax_bwd: W is not the forward's")
+    if (dx and not state.want & RS_CATALOG_DX) or (dw and not state.want & RS_CATALOG_DW):
+        raise ValueError("catalog_softmax_bwd: the forward was not asked for this gradient (want_grad)")
+    if g is not None and (_dev(g, "g").numel() != 1 or g.device != W.device):
+        raise ValueError("catalog_softmax_bwd: g must be one float32 value on W's device")
+    W = _aligned(W)
+    dev, dt, want = W.device, RS_DTYPES[state.dtype], state.want
+    with torch.cuda.device(dev):
+        dX = torch.empty((state.N, state.D), dtype=state.dtype, device=dev) if dx else None
+        dW = torch.empty((state.V, state.D), dtype=state.dtype, device=dev) if dw else None
+        ws = _ws(query("rs_catalog_softmax_workspace_bytes", state.N, state.V, state.D, dt, want), dev)
+        call("rs_catalog_softmax_bwd", _p(W), state.N, state.V, state.D, dt, state.scale, want, _p(g), _p(state.keep),
+             state.keep.numel(), _p(dX), _p(dW), _p(ws), ws.numel(), _stream())
+    return dX, dW
+
+
+def dropout_state(seed: int, device=None) -> torch.Tensor:
+    """A dropout generator on the device: int64 [2] = (seed, step), advanced by dropout_ticket."""
+    return torch.tensor([int(seed), 0], dtype=torch.int64, device=device or torch.device("cuda"))
+
+
+def _ticket_check(t, name):
+    if _dev(t, name, torch.int64).numel() != 2:
+        raise ValueError(f"{name}: expected int64 [2] = (seed, step)")
+    return t
+
+
+def dropout_ticket(state: torch.Tensor) -> torch.Tensor:
+    """The (seed, step) of the next mask: a copy of the state, whose step is then advanced (on the
+    device: a captured step draws a new mask at each replay)."""
+    _ticket_check(state, "state")
+    with torch.cuda.device(state.device):
+        ticket = torch.empty((2,), dtype=torch.int64, device=state.device)
+        call("rs_dropout_ticket", _p(state), _p(ticket), _stream())
+    return ticket
+
+
+def dropout_apply(x: torch.Tensor, rate: float, ticket: torch.Tensor, out: Optional[torch.Tensor] = None):
+    """x / (1 - rate) where the element's Philox word under `ticket` (seed, step) is at least
+    round(rate 2^32), else 0 (rs_dropout). The gradient is the same call on it with the same ticket.
+    float32 or bfloat16; out may be x."""
+    x = x.detach()
+    _dev_typed(x, "x"), _ticket_check(ticket, "ticket")
+    if not 0.0 <= rate < 1.0:
+        raise ValueError(f"dropout: rate must lie in [0, 1), got {rate!r}")
+    if ticket.device != x.device:
+        raise ValueError("dropout: x and ticket must be on one device")
+    with torch.cuda.device(x.device):
+        if out is None:
+            out = torch.empty_like(x)
+        elif _dev(out, "out", x.dtype).shape != x.shape or out.device != x.device:
+            raise ValueError("dropout: out must match x")
+        call("rs_dropout", _p(x), x.numel(), RS_DTYPES[x.dtype], float(rate), _p(ticket), _p(out), _stream())
+    return out
+
+
+# --------------------------------------------------------------------------------------------
 # autograd Functions
 # --------------------------------------------------------------------------------------------
 class SparseGradSink:
@@ -2185,3 +2328,55 @@ class L2PenaltyFn(torch.autograd.Function):
     def backward(ctx, g):
         ws = ctx.saved_tensors
         return (None, *[w * (2.0 * ctx.l2) * g for w in ws])
+
+
+class CatalogSoftmaxFn(torch.autograd.Function):
+    """catalog_softmax_fwd / _bwd as a node: apply(X, W, labels, weights, scale, ignore_index,
+    reduction) -> (loss, row_loss); the per-row losses are non-differentiable (use weights)."""
+
+    @staticmethod
+    def forward(ctx, X, W, labels, weights, scale: float, ignore_index: int, reduction: str):
+        ctx.set_materialize_grads(False)
+        W = W.contiguous()
+        loss, row, _, ctx.state = catalog_softmax_fwd(
+            X.contiguous(), W, labels.contiguous(), scale, weights.contiguous() if weights is not None else None,
+            ignore_index, reduction, want_grad=(ctx.needs_input_grad[0], ctx.needs_input_grad[1]))
+        ctx.save_for_backward(W)
+        ctx.mark_non_differentiable(row)
+        return loss, row
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g, _g_row):
+        if g is None:
+            return (None,) * 7
+        W, = ctx.saved_tensors
+        dX, dW = catalog_softmax_bwd(W, ctx.state, g.contiguous(), ctx.needs_input_grad[0], ctx.needs_input_grad[1])
+        return dX, dW, None, None, None, None, None
+
+
+def catalog_softmax_loss(X, W, labels, scale: float = 1.0, weights=None, ignore_index: int = -100,
+                         reduction: str = "sum"):
+    """(loss, row_loss) of catalog_softmax_fwd, differentiable by X and W through the loss."""
+    return CatalogSoftmaxFn.apply(X, W, labels, weights, float(scale), int(ignore_index), reduction)
+
+
+class DropoutFn(torch.autograd.Function):
+    """dropout_apply as a node: the backward makes the mask again from the saved ticket."""
+
+    @staticmethod
+    def forward(ctx, x, rate: float, ticket):
+        ctx.rate = rate
+        ctx.save_for_backward(ticket)
+        return dropout_apply(x.contiguous(), rate, ticket)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        ticket, = ctx.saved_tensors
+        return dropout_apply(dy.contiguous(), ctx.rate, ticket), None, None
+
+
+def dropout(x: torch.Tensor, rate: float, ticket: torch.Tensor) -> torch.Tensor:
+    """Dropout of x with the mask of `ticket` (dropout_ticket, or an int64 [2] (seed, step) tensor)."""
+    return DropoutFn.apply(x, float(rate), ticket)
