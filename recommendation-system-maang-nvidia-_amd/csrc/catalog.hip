@@ -46,6 +46,8 @@ struct CsScal {
   float w_inv;   // 2^-e of the catalogue's scale (fp32), 1 (bf16)
   float c0;      // -exponent of the largest |a_n| / x-scale (fp32): keeps p a in fp16's range
   float inv_z;   // 1 / Z of the reduction
+  float pad;
+  float zero[4];  // 16 zero bytes, for the columns past a width
 };
 
 // row statistics the column pass streams beside x: per 32 rows four arrays of 32 words
@@ -57,15 +59,18 @@ struct CsPass {
   const char* T;          // streamed rows [nT][D]
   int64_t nR, nT, t_last; // valid rows; the last streamed row that may be read
   int64_t r_plane, t_plane;
+  int64_t r_ld, t_ld;     // bytes per row
+  int r_ch, t_ch;         // 16-byte chunks a row holds (the rest of the kernel's width reads as zero)
+  const char* zero;       // 16 zero bytes
   int64_t tiles, per;     // streamed tiles, tiles per split
-  int nrb;                // resident blocks
+  int nrb, nsplit;        // resident blocks, splits
   const CsScal* scal;
   float scale, kbase;     // c, c log2 e
   const float* kx;        // row pass, fp32: 2^-e of each resident row
   const int32_t* lab;     // row pass: label of each resident row (< 0: none)
   const float* stat;      // column pass: statistics of the streamed rows
   const float* lq;        // column pass: log2 q of the streamed rows
-  float *m, *l, *O;       // partials [split][nR](, [D])
+  float *m, *l, *O;       // partials m, l [nR][split], O [split][nR][D]
   // column pass, one split: the gradient itself
   void* out;
   int64_t ld;             // its row length (0: partials)
@@ -80,14 +85,11 @@ __device__ __forceinline__ f32x4 cs_mfma(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(cs_h8, a), __builtin_bit_cast(cs_h8, b), c, 0, 0, 0);
 }
 
-// 16-B chunk ch of tile row r lies at chunk ch ^ cs_swz(r) of its LDS row: both the row reads (16 rows
-// 8 a + b + const, one chunk each) and the transposed reads (16 rows, one chunk pair) then touch every
-// bank evenly; bit 2 of the row does not enter, so rows r and r + 4 differ by an immediate.
-template <int D>
-__device__ __forceinline__ int cs_swz(int r) {
-  if constexpr (D == 64) return (((r >> 1) & 1) << 2) | (((r >> 3) & 1) << 1) | ((r >> 4) & 1);
-  else return ((r & 3) << 2) | (((r >> 3) & 1) << 1) | ((r >> 4) & 1);
-}
+// LDS image of a tile: bands of 8 rows, each D / 32 subtiles of 8 rows x 64 bytes; the four 16-B chunks of
+// a subtile row are permuted by XOR with cs_swz(band). The row reads (16 rows of two or four bands, one
+// chunk) and the transposed reads (16 rows, 32 bytes) then touch every bank evenly, and each kind needs
+// one or two per-lane addresses, the rest being instruction offsets.
+__device__ __forceinline__ int cs_swz(int band) { return ((((band) ^ (band >> 1)) & 1) << 1) | ((band >> 1) & 1); }
 
 // 16 B per lane from global memory to LDS at dst + 16 lane (dst uniform); only an explicit vmcnt waits
 // for it
@@ -114,44 +116,88 @@ __device__ __forceinline__ int cs_xcd(int id, int n) {
 
 enum { CS_STATS = 0, CS_ROW = 1, CS_COL = 2 };
 
-// Register and LDS budget: 8 waves of 32 resident rows (two per SIMD, 256 registers) up to D = 128;
-// D = 256 fp32 holds x's two planes and O in 512 registers, one wave per SIMD.
-constexpr int cs_waves(int D) { return D == 256 ? 4 : 8; }
-constexpr int CS_UB = 2;   // 16-row subtiles of resident rows per wave
-constexpr int CS_KT = 64;  // streamed rows per tile
-constexpr int cs_block_rows(int D) { return 16 * CS_UB * cs_waves(D); }
+// Shape of a pass: UB 16-row subtiles of resident rows per wave, NW waves, tiles of 64 streamed rows taken
+// in groups of 32 SG rows, NB tiles in LDS; LAG: a group's second product runs beside the next group's
+// exponentials.
+#ifndef CS_V
+#define CS_V 0
+#endif
+struct CsCfg {
+  int UB, NW, KT, NB, SG;
+  bool LAG;
+};
+constexpr CsCfg cs_cfg(int D, int NP, int MODE) {
+  if (D == 256) return CS_V == 1 ? CsCfg{1, 8, 32, 4, 1, true} : CS_V == 2 ? CsCfg{1, 8, 32, 4, 1, false} : CsCfg{1, 8, 64, 2, 2, false};
+  if (CS_V == 1) return {2, 8, 64, 3, 1, true};
+  if (CS_V == 2) return {2, 8, 64, 3, 1, false};
+  if (CS_V == 3) return {2, 4, 64, 2, 2, false};
+  return {2, 8, 64, 2, 2, false};
+}
+constexpr int cs_block_rows(int D, int NP, int MODE) {
+  return 16 * cs_cfg(D, NP, MODE).UB * cs_cfg(D, NP, MODE).NW;
+}
+
+// waves per SIMD the registers are budgeted for
+constexpr int cs_lb(int D, int NP, int MODE) { return D == 256 && cs_cfg(D, NP, MODE).UB == 2 ? 1 : 2; }
+
+template <int N>
+__device__ __forceinline__ void cs_wait() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"i"(N) : "memory");
+}
 
 template <int D, int NP, int MODE>
-__global__ __launch_bounds__(64 * cs_waves(D), cs_waves(D) / 4) void cs_pass_kernel(CsPass p) {
-  constexpr int UB = CS_UB, NW = cs_waves(D), KT = CS_KT;
-  constexpr int CH = D / 8, ROWB = 2 * D, PLANE = KT * ROWB, IMG = NP * PLANE, NS = KT / 32, NDT = D / 16, NC = D / 32;
-  constexpr int STAT = MODE == CS_COL ? KT * 16 : 0;
+__global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) void cs_pass_kernel(CsPass p) {
+  constexpr int UB = cs_cfg(D, NP, MODE).UB, NW = cs_cfg(D, NP, MODE).NW, KT = cs_cfg(D, NP, MODE).KT;
+  constexpr int NB = cs_cfg(D, NP, MODE).NB;
+  constexpr int ROWB = 2 * D, PLANE = KT * ROWB, IMG = NP * PLANE, NS = KT / 32, NDT = D / 16, NC = D / 32;
+  constexpr int STAT = MODE == CS_COL ? KT * 16 : 0, BUF = IMG + STAT;
   constexpr bool RUNMAX = MODE != CS_COL || NP == 2;
-  __shared__ __attribute__((aligned(1024))) char smem[2 * (IMG + STAT)];
+  __shared__ __attribute__((aligned(1024))) char smem[NB * BUF];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4, i16 = lane & 15;
   const int id = cs_xcd(blockIdx.x, gridDim.x);
   const int split = id / p.nrb;
-  const int64_t r0 = (int64_t)(id % p.nrb) * cs_block_rows(D) + wave * (16 * UB);
+  const int64_t r0 = (int64_t)(id % p.nrb) * cs_block_rows(D, NP, MODE) + wave * (16 * UB);
   const int64_t tb0 = split * p.per, tb1 = tb0 + p.per < p.tiles ? tb0 + p.per : p.tiles;
   const uint32_t lds0 = (uint32_t) reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)smem);
 
-  auto copy = [&](int64_t t, int buf) __attribute__((always_inline)) {
-    const int64_t row0 = t * KT;
+  constexpr int SG = cs_cfg(D, NP, MODE).SG;
+  constexpr bool LAG = cs_cfg(D, NP, MODE).LAG;
+  constexpr int CPT = PLANE / (NW * 1024);    // 16-B copies per thread and plane of a tile
+  constexpr int AHEAD = LAG ? NB - 2 : NB - 1;  // tiles copied ahead (see the loop)
+  static_assert(CPT >= 1 && KT % (32 * SG) == 0 && AHEAD >= 1 && (!LAG || MODE == CS_STATS || SG == 1), "tile shape");
+  // this thread's copies of the next tile; a chunk past the rows' width comes from the zeros
+  const char* src[CPT];
+  int64_t src_step[CPT];
 #pragma unroll
-    for (int i = 0; i < PLANE / (NW * 1024); ++i) {
-      const int row = i * (NW * 64 / CH) + tid / CH;
-      const int ch = (tid % CH) ^ cs_swz<D>(row);
-      const int64_t rr = row0 + row < p.t_last ? row0 + row : p.t_last;
-      const char* s = p.T + rr * ROWB + ch * 16;
+  for (int i = 0; i < CPT; ++i) {
+    const int at = i * NW * 64 + tid, band = at / D;  // 16-B chunk of the image
+    const int row = band * 8 + (at % 32) / 4, ch = (at % D) / 32 * 4 + ((at & 3) ^ cs_swz(band & 3));
+    src[i] = ch < p.t_ch ? p.T + (tb0 * KT + row) * p.t_ld + ch * 16 : p.zero;
+    src_step[i] = ch < p.t_ch ? KT * p.t_ld : 0;
+  }
+  auto copy = [&](int64_t t, int buf) __attribute__((always_inline)) {
+    const int64_t over = t * KT + KT - 1 - p.t_last;  // rows of the tile past the last one repeat it
+#pragma unroll
+    for (int i = 0; i < CPT; ++i) {
+      const char* q = src[i];
+      if (over > 0) {
+        const int row = (i * NW * 64 + tid) / D * 8 + ((i * NW * 64 + tid) % 32) / 4;
+        const int64_t back = row + over - (KT - 1);
+        if (back > 0 && src_step[i]) q -= back * p.t_ld;
+      }
 #pragma unroll
       for (int pl = 0; pl < NP; ++pl)
-        cs_glds16(s + pl * p.t_plane, lds0 + buf * (IMG + STAT) + pl * PLANE + i * NW * 1024 + wave * 1024);
+        cs_glds16(q + pl * p.t_plane, lds0 + buf * BUF + pl * PLANE + i * NW * 1024 + wave * 1024);
+      src[i] += src_step[i];
     }
     if constexpr (MODE == CS_COL)
-      if (wave == 0) cs_glds16((const char*)p.stat + row0 * 16 + lane * 16, lds0 + buf * (IMG + STAT) + IMG);
+      if (wave == 0 && lane < KT)
+        cs_glds16((const char*)p.stat + t * (KT * 16) + lane * 16, lds0 + buf * BUF + IMG);
   };
-  if (tb0 < tb1) copy(tb0, 0);
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i)
+    if (tb0 + i < tb1) copy(tb0 + i, i);
 
   // resident rows as the B operand: column i16 of subtile ub, k = 32 c + 8 g ..
   u32x4 xq[UB][NC][NP];
@@ -165,31 +211,33 @@ __global__ __launch_bounds__(64 * cs_waves(D), cs_waves(D) / 4) void cs_pass_ker
     for (int c = 0; c < NC; ++c)
 #pragma unroll
       for (int pl = 0; pl < NP; ++pl)
-        xq[ub][c][pl] = *reinterpret_cast<const u32x4*>(p.R + pl * p.r_plane + q * ROWB + (4 * c + g) * 16);
+        xq[ub][c][pl] = *reinterpret_cast<const u32x4*>(
+            4 * c + g < p.r_ch ? p.R + pl * p.r_plane + q * p.r_ld + (4 * c + g) * 16 : p.zero);
     if constexpr (MODE != CS_COL) {
       // FLT_MIN: a masked item's -inf must stay -inf after the product
       kq[ub] = NP == 2 ? fminf(fmaxf(p.kbase * p.scal->w_inv * p.kx[q], FLT_MIN), FLT_MAX) : p.kbase;
       lab[ub] = p.lab[q];
     }
   }
-  const float kw = NP == 2 ? p.kbase * p.scal->w_inv : p.kbase;
+  // the resident rows are waited for here: a wait inside the loop would also wait for every copy in flight
+#pragma unroll
+  for (int ub = 0; ub < UB; ++ub) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int pl = 0; pl < NP; ++pl) asm volatile("" : "+v"(xq[ub][c][pl]));
+    if constexpr (MODE != CS_COL) asm volatile("" : "+v"(kq[ub]), "+v"(lab[ub]));
+  }
+  const float kw = p.kbase;
   const float ps = NP == 2 ? (MODE == CS_COL ? CS_PS + p.scal->c0 : CS_PS) : 0.f;
 
-  // row reads: A row i16 of subtile (s, kb) = tile row 32 s + 4 kb + 8 (i16 / 4) + i16 % 4, chunk 4 c + g
-  uint32_t ab[NC < 4 ? NC : 4];
-  {
-    const int rho = 8 * (i16 >> 2) + (i16 & 3);
+  // row reads: A row i16 of subtile kb = row 8 (i16 / 4) + 4 kb + i16 % 4 of 32, chunk 4 c + g
+  const uint32_t ab = lds0 + (i16 >> 2) * (8 * ROWB) + (i16 & 3) * 64 + (g ^ cs_swz(i16 >> 2)) * 16;
+  // transposed reads: row 8 g + 4 h + i16 / 4 of 32, columns 16 dt + 4 (i16 % 4) .., by dt % 2
+  uint32_t tb[2];
 #pragma unroll
-    for (int c = 0; c < (NC < 4 ? NC : 4); ++c) ab[c] = lds0 + rho * ROWB + (((4 * c + g) ^ cs_swz<D>(rho)) * 16);
-  }
-  // transposed reads: tile row 32 s + 8 g + 4 h + i16 / 4, columns 16 dt + 4 (i16 % 4) ..
-  uint32_t tb[NDT < 8 ? NDT : 8];
-  {
-    const int rho = 8 * g + (i16 >> 2), pp = i16 & 3;
-#pragma unroll
-    for (int dt = 0; dt < (NDT < 8 ? NDT : 8); ++dt)
-      tb[dt] = lds0 + rho * ROWB + (((2 * dt + (pp >> 1)) ^ cs_swz<D>(rho)) * 16) + 8 * (pp & 1);
-  }
+  for (int o = 0; o < 2; ++o)
+    tb[o] = lds0 + g * (8 * ROWB) + (i16 >> 2) * 64 + ((2 * o + ((i16 & 3) >> 1)) ^ cs_swz(g)) * 16 + 8 * (i16 & 1);
 
   f32x4 O[MODE == CS_STATS ? 1 : NDT][UB];
 #pragma unroll
@@ -202,194 +250,306 @@ __global__ __launch_bounds__(64 * cs_waves(D), cs_waves(D) / 4) void cs_pass_ker
     m[ub] = CS_MIN;
     l[ub] = 0.f;
   }
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  __syncthreads();
+  struct Scores {
+    f32x4 v[2 * SG][UB];  // [2 sub + kb][ub]: streamed row 32 sub + 8 g + 4 kb + r, resident row 16 ub + i16
+  };
+  struct Probs {
+    u32x4 w[SG][UB][NP];  // the second product's B operand: k = 8 g + j of sub, j < 4 from kb = 0
+  };
 
-  for (int64_t t = tb0; t < tb1; ++t) {
-    const int buf = (int)(t - tb0) & 1;
-    const uint32_t bo = buf * (IMG + STAT);
-    if (t + 1 < tb1) copy(t + 1, buf ^ 1);
-
-    f32x4 s[2 * NS][UB];  // [2 sub + kb][ub]: streamed row 32 sub + 8 g + 4 kb + r, resident 16 ub + i16
+  // S of the group's streamed rows at LDS byte bo; the next k step's rows are read ahead of this one's products
+  auto scores = [&](uint32_t bo, Scores& s) __attribute__((always_inline)) {
+    uint32_t at = ab + bo;
+    asm("" : "+v"(at));  // the offsets below stay in the instructions
+    constexpr int NST = SG * NC;
+    u32x4 a[2][2][NP];
+    auto read = [&](int j) __attribute__((always_inline)) {
 #pragma unroll
-    for (int k = 0; k < 2 * NS; ++k)
-#pragma unroll
-      for (int ub = 0; ub < UB; ++ub) s[k][ub] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int c = 0; c < NC; ++c)
-#pragma unroll
-      for (int k = 0; k < 2 * NS; ++k) {
-        u32x4 a[NP];
+      for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
         for (int pl = 0; pl < NP; ++pl)
-          a[pl] = cs_lds<u32x4>(ab[c & 3] + bo + (c >> 2) * 256 + (32 * (k >> 1) + 4 * (k & 1)) * ROWB + pl * PLANE);
+          a[j & 1][kb][pl] = cs_lds<u32x4>(at + (j / NC) * (32 * ROWB) + (j % NC) * 512 + kb * 256 + pl * PLANE);
+    };
+    read(0);
+#pragma unroll
+    for (int j = 0; j < NST; ++j) {
+      const int c = j % NC;
+      if (j + 1 < NST) read(j + 1);
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
         for (int ub = 0; ub < UB; ++ub) {
+          f32x4& o = s.v[2 * (j / NC) + kb][ub];
+          f32x4 z = {0.f, 0.f, 0.f, 0.f};
+          if (c > 0) z = o;
           if constexpr (NP == 2) {
-            s[k][ub] = cs_mfma<NP>(a[1], xq[ub][c][0], s[k][ub]);
-            s[k][ub] = cs_mfma<NP>(a[0], xq[ub][c][1], s[k][ub]);
+            z = cs_mfma<NP>(a[j & 1][kb][1], xq[ub][c][0], z);
+            z = cs_mfma<NP>(a[j & 1][kb][0], xq[ub][c][1], z);
           }
-          s[k][ub] = cs_mfma<NP>(a[0], xq[ub][c][0], s[k][ub]);
+          o = cs_mfma<NP>(a[j & 1][kb][0], xq[ub][c][0], z);
         }
-      }
-
-    bool hit = false;  // a label's element lies in this tile (uniform)
-    if constexpr (MODE == CS_COL) {
-      // log2 p = s k_n - lse2_n
-#pragma unroll
-      for (int k = 0; k < 2 * NS; ++k) {
-        const uint32_t sb = lds0 + bo + IMG + (k >> 1) * 512 + (8 * g + 4 * (k & 1)) * 4;
-        const f32x4 ls = cs_lds<f32x4>(sb + CS_LSE2 * 128);
-        f32x4 kn = f32x4{kw, kw, kw, kw};
-        if constexpr (NP == 2) kn = cs_lds<f32x4>(sb + CS_KX * 128);
-#pragma unroll
-        for (int ub = 0; ub < UB; ++ub)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) s[k][ub][r] = __builtin_fmaf(s[k][ub][r], kn[r], -ls[r]);
-      }
-      const int32_t lb = cs_lds<int32_t>(lds0 + bo + IMG + (lane >> 5) * 512 + CS_LAB * 128 + (lane & 31) * 4);
-      hit = __any((uint32_t)(lb - (int32_t)r0) < (uint32_t)(16 * UB));
-      if (hit) {
-#pragma unroll
-        for (int k = 0; k < 2 * NS; ++k) {
-          const int n4 = 8 * g + 4 * (k & 1);
-          const int64_t row = t * KT + 32 * (k >> 1) + n4;
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int32_t ln = cs_lds<int32_t>(lds0 + bo + IMG + (k >> 1) * 512 + CS_LAB * 128 + (n4 + r) * 4);
-            const float lqn = p.lq[row + r];
-#pragma unroll
-            for (int ub = 0; ub < UB; ++ub)
-              if (ln == (int32_t)r0 + 16 * ub + i16) s[k][ub][r] = lqn;
-          }
-        }
-      }
-    } else {
-      const int64_t v0 = t * KT;
-      bool mine = false;
-#pragma unroll
-      for (int ub = 0; ub < UB; ++ub) mine |= (uint32_t)(lab[ub] - (int32_t)v0) < (uint32_t)KT;
-      if (__any(mine) || v0 + KT > p.nT) {
-#pragma unroll
-        for (int k = 0; k < 2 * NS; ++k)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int64_t v = v0 + 32 * (k >> 1) + 8 * g + 4 * (k & 1) + r;
-#pragma unroll
-            for (int ub = 0; ub < UB; ++ub)
-              if (v >= p.nT || (int32_t)v == lab[ub]) s[k][ub][r] = -INFINITY;
-          }
-      }
+      __builtin_amdgcn_sched_barrier(0);
     }
-
-    if constexpr (RUNMAX) {
-      float mx[UB];
-      bool up = false;
+  };
+  // O += P times the group's rows, beside(dt) placed with each column tile's instructions. fp32 operands:
+  // the group's sum in fresh accumulators, then one fp32 multiply-add that also brings O to the scale P
+  // was formed at.
+  auto product = [&](uint32_t bo, const Probs& pb, const float (&al)[UB], auto&& beside) __attribute__((always_inline)) {
+    uint32_t at[2] = {tb[0] + bo, tb[1] + bo};
+    asm("" : "+v"(at[0]), "+v"(at[1]));
+    constexpr int NST = SG * NDT;
+    u32x4 a[2][NP];
+    f32x4 f[UB];
+    auto read = [&](int j) __attribute__((always_inline)) {
+      const int dt = j / SG;
+#pragma unroll
+      for (int pl = 0; pl < NP; ++pl)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const ib_s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (__attribute__((address_space(3))) ib_s16x4*)(uintptr_t)(at[dt & 1] + (j % SG) * (32 * ROWB) +
+                                                                       (dt >> 1) * 512 + h * 256 + pl * PLANE));
+          const u32x2 w2 = __builtin_bit_cast(u32x2, v);
+          a[j & 1][pl][2 * h] = w2[0];
+          a[j & 1][pl][2 * h + 1] = w2[1];
+        }
+    };
+    read(0);
+#pragma unroll
+    for (int j = 0; j < NST; ++j) {
+      const int dt = j / SG, sub = j % SG;
+      if (j + 1 < NST) read(j + 1);
 #pragma unroll
       for (int ub = 0; ub < UB; ++ub) {
-        mx[ub] = fmaxf(s[0][ub][0], s[0][ub][1]);
-#pragma unroll
-        for (int k = 0; k < 2 * NS; ++k)
-#pragma unroll
-          for (int r = k == 0 ? 2 : 0; r < 4; r += 2) mx[ub] = fmaxf(fmaxf(s[k][ub][r], s[k][ub][r + 1]), mx[ub]);
-        mx[ub] = (MODE == CS_COL ? mx[ub] : mx[ub] * kq[ub]) - ps;
-        up |= mx[ub] > m[ub];
+        if constexpr (NP == 2) {
+          if (sub == 0) f[ub] = f32x4{0.f, 0.f, 0.f, 0.f};
+          f[ub] = cs_mfma<NP>(a[j & 1][1], pb.w[sub][ub][0], f[ub]);
+          f[ub] = cs_mfma<NP>(a[j & 1][0], pb.w[sub][ub][1], f[ub]);
+          f[ub] = cs_mfma<NP>(a[j & 1][0], pb.w[sub][ub][0], f[ub]);
+          if (sub == SG - 1) O[dt][ub] = O[dt][ub] * al[ub] + f[ub];
+        } else {
+          O[dt][ub] = cs_mfma<NP>(a[j & 1][0], pb.w[sub][ub][0], O[dt][ub]);
+        }
       }
-      if (__any(up)) {
+      if (sub == 0) beside(dt);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  // four probabilities of subtile k -> words of P
+  auto pack = [&](Probs& pb, int k, int ub, f32x4 e) __attribute__((always_inline)) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float a = e[2 * h], b = e[2 * h + 1];
+      const int w = 2 * (k & 1) + h;
+      if constexpr (NP == 1) pb.w[k >> 1][ub][0][w] = ib_pk(a, b);
+      else {
+        const cs_h2 hi = __builtin_bit_cast(cs_h2, __builtin_amdgcn_cvt_pkrtz(a, b));
+        pb.w[k >> 1][ub][0][w] = __builtin_bit_cast(uint32_t, hi);
+        pb.w[k >> 1][ub][1][w] =
+            __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a - (float)hi[0], b - (float)hi[1]));
+      }
+    }
+  };
+  auto stat_at = [&](uint32_t st, int a, int k) __attribute__((always_inline)) {
+    return st + (k >> 1) * 512 + a * 128 + (8 * g + 4 * (k & 1)) * 4;
+  };
+  // f(k, ub, r, whether this element is its streamed row's label, log2 q of that row)
+  auto each_hit = [&](int64_t n0, uint32_t st, auto&& f) __attribute__((always_inline)) {
+#pragma unroll
+    for (int k = 0; k < 2 * SG; ++k)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int32_t at = cs_lds<int32_t>(stat_at(st, CS_LAB, k) + 4 * r) - ((int32_t)r0 + i16);
+        const float lq = p.lq[n0 + 32 * (k >> 1) + 8 * g + 4 * (k & 1) + r];
+#pragma unroll
+        for (int ub = 0; ub < UB; ++ub) f(k, ub, r, at == 16 * ub, lq);
+      }
+  };
+  // Before a group's exponentials (its first streamed row is n0): the label's term leaves them and the
+  // running maximum is raised (up, al: what that multiplies O and l by). Both are rare, and what they
+  // change is small, so the common path has no branch between its matrix and vector instructions.
+  auto prepare = [&](int64_t n0, uint32_t st, Scores& s, float (&al)[UB], bool& up, bool& hit) __attribute__((always_inline)) {
+    up = hit = false;
+    if constexpr (MODE == CS_COL) {
+      if constexpr (NP == 2) {
+        // log2 p = s k_n - lse2_n
+#pragma unroll
+        for (int k = 0; k < 2 * SG; ++k) {
+          const f32x4 ls = cs_lds<f32x4>(stat_at(st, CS_LSE2, k)), kn = cs_lds<f32x4>(stat_at(st, CS_KX, k));
+#pragma unroll
+          for (int ub = 0; ub < UB; ++ub)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s.v[k][ub][r] = __builtin_fmaf(s.v[k][ub][r], kn[r], -ls[r]);
+        }
+      }
+      const int ll = lane & (32 * SG - 1);
+      const int32_t lb = cs_lds<int32_t>(st + (ll >> 5) * 512 + CS_LAB * 128 + (ll & 31) * 4);
+      hit = __any((uint32_t)(lb - (int32_t)r0) < (uint32_t)(16 * UB));
+      if (hit) each_hit(n0, st, [&](int k, int ub, int r, bool is, float lq) __attribute__((always_inline)) {
+        s.v[k][ub][r] = is ? (NP == 2 ? lq : -INFINITY) : s.v[k][ub][r];
+      });
+    } else {
+      bool mine = false;
+#pragma unroll
+      for (int ub = 0; ub < UB; ++ub) mine |= (uint32_t)(lab[ub] - (int32_t)n0) < 32u * SG;
+      if (__any(mine) || n0 + 32 * SG > p.nT) {
+        const int32_t base = (int32_t)n0 + 8 * g, left = (int32_t)p.nT - base;
+#pragma unroll
+        for (int ub = 0; ub < UB; ++ub) {
+          const int32_t at = lab[ub] - base;
+#pragma unroll
+          for (int k = 0; k < 2 * SG; ++k)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const int v = 32 * (k >> 1) + 4 * (k & 1) + r;
+              s.v[k][ub][r] = v >= left || v == at ? -INFINITY : s.v[k][ub][r];
+            }
+        }
+      }
+    }
+#pragma unroll
+    for (int ub = 0; ub < UB; ++ub) al[ub] = 1.f;
+    if constexpr (RUNMAX) {
+      float mx[UB];
+      bool mine = false;
+#pragma unroll
+      for (int ub = 0; ub < UB; ++ub) {
+        float z = fmaxf(s.v[0][ub][0], s.v[0][ub][1]);
+#pragma unroll
+        for (int k = 0; k < 2 * SG; ++k)
+#pragma unroll
+          for (int r = k == 0 ? 2 : 0; r < 4; r += 2) z = fmaxf(fmaxf(s.v[k][ub][r], s.v[k][ub][r + 1]), z);
+        mx[ub] = (MODE == CS_COL ? z : z * kq[ub]) - ps;
+        mine |= mx[ub] > m[ub];
+      }
+      up = __any(mine);
+      if (up) {
 #pragma unroll
         for (int ub = 0; ub < UB; ++ub) {
           float x = fmaxf(mx[ub], __shfl_xor(mx[ub], 16, 64));
           x = fmaxf(x, __shfl_xor(x, 32, 64));
           x = fmaxf(x, m[ub]);
-          const float al = __builtin_amdgcn_exp2f(m[ub] - x);
+          al[ub] = __builtin_amdgcn_exp2f(m[ub] - x);
           m[ub] = x;
-          l[ub] *= al;
-          if constexpr (MODE != CS_STATS)
-#pragma unroll
-            for (int dt = 0; dt < NDT; ++dt) O[dt][ub] *= al;
+          l[ub] *= al[ub];
         }
       }
     }
+  };
+  // the label's element of P: -q a (its exponential is not wanted there)
+  auto patch = [&](int64_t n0, uint32_t st, Probs& pb) __attribute__((always_inline)) {
+    each_hit(n0, st, [&](int k, int ub, int r, bool is, float lq) __attribute__((always_inline)) {
+      const float cf = cs_lds<float>(stat_at(st, CS_COEF, k) + 4 * r);
+      const float e = -cf * __builtin_amdgcn_exp2f(NP == 2 ? lq - m[ub] : lq);
+      Probs one;
+      pack(one, k, ub, f32x4{e, e, e, e});
+      const uint32_t mask = r & 1 ? 0xffff0000u : 0xffffu;
+      const int at = 2 * (k & 1) + (r >> 1);
+#pragma unroll
+      for (int pl = 0; pl < NP; ++pl) {
+        const uint32_t w = pb.w[k >> 1][ub][pl][at];
+        pb.w[k >> 1][ub][pl][at] = is ? (w & ~mask) | (one.w[k >> 1][ub][pl][at] & mask) : w;
+      }
+    });
+  };
+  // exponentials of part i = (subtile k, ub) of 2 SG UB
+  auto exponentials = [&](int i, uint32_t st, const Scores& s, Probs& pb) __attribute__((always_inline)) {
+    const int k = i / UB, ub = i % UB;
+    f32x4 cf, ls, e;
+    if constexpr (MODE == CS_COL) cf = cs_lds<f32x4>(stat_at(st, CS_COEF, k));
+    if constexpr (MODE == CS_COL && NP == 1) ls = cs_lds<f32x4>(stat_at(st, CS_LSE2, k));
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const float x = s.v[k][ub][r];
+      if constexpr (MODE != CS_COL) e[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x, kq[ub], -m[ub]));
+      else if constexpr (NP == 2) e[r] = __builtin_amdgcn_exp2f(x - m[ub]) * cf[r];
+      else e[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x, kw, -ls[r])) * cf[r];
+    }
+    if constexpr (MODE != CS_COL) l[ub] += (e[0] + e[1]) + (e[2] + e[3]);
+    if constexpr (MODE != CS_STATS) pack(pb, k, ub, e);
+  };
+  // O and l follow a raised maximum (bf16; with fp32 operands the product does it for O)
+  auto rescale = [&](bool up, const float (&al)[UB]) __attribute__((always_inline)) {
+    if constexpr (NP == 1 && MODE == CS_ROW)
+      if (up)
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+          for (int ub = 0; ub < UB; ++ub) O[dt][ub] *= al[ub];
+  };
+  struct Pending {  // LAG: the previous group's P, not yet in O
+    Probs pb;
+    uint32_t bo = 0;
+    float al[UB];
+    bool up = false;
+  } pend;
+#pragma unroll
+  for (int ub = 0; ub < UB; ++ub) {
+    pend.al[ub] = 1.f;
+#pragma unroll
+    for (int sub = 0; sub < SG; ++sub)
+#pragma unroll
+      for (int pl = 0; pl < NP; ++pl) pend.pb.w[sub][ub][pl] = u32x4{0, 0, 0, 0};
+  }
+  auto group = [&](int64_t n0, uint32_t bo, uint32_t st) __attribute__((always_inline)) {
+    constexpr int PARTS = 2 * SG * UB;
+    float al[UB];
+    bool up, hit;
+    Scores s;
+    Probs pb;
+    scores(bo, s);
+    prepare(n0, st, s, al, up, hit);
+    if constexpr (!LAG || MODE == CS_STATS) {
+      rescale(up, al);
+#pragma unroll
+      for (int i = 0; i < PARTS; ++i) exponentials(i, st, s, pb);
+    } else {
+      rescale(pend.up, pend.al);
+      product(pend.bo, pend.pb, pend.al, [&](int dt) __attribute__((always_inline)) {
+        if (dt % (NDT / PARTS) == 0) exponentials(dt / (NDT / PARTS), st, s, pb);
+      });
+      // keeps the exponentials here: P is used in the next group only, and would sink there
+#pragma unroll
+      for (int ub = 0; ub < UB; ++ub)
+#pragma unroll
+        for (int pl = 0; pl < NP; ++pl) asm volatile("" : "+v"(pb.w[0][ub][pl]));
+    }
+    if (MODE == CS_COL && hit) {
+      asm volatile("");  // keeps the rare path a branch
+      patch(n0, st, pb);
+    }
+    if constexpr (!LAG && MODE != CS_STATS) product(bo, pb, al, [](int) {});
+    if constexpr (LAG) {
+      pend.pb = pb;
+      pend.bo = bo;
+      pend.up = up;
+#pragma unroll
+      for (int ub = 0; ub < UB; ++ub) pend.al[ub] = al[ub];
+    }
+  };
 
-    // exponentials; P's words are the second product's B operand: k = 8 g + j of sub = [2 sub][j], j < 4,
-    // [2 sub + 1][j - 4]
-    u32x4 pb[MODE == CS_STATS ? 1 : NS][UB][NP];
-#pragma unroll
-    for (int k = 0; k < 2 * NS; ++k) {
-      f32x4 cf;
-      if constexpr (MODE == CS_COL)
-        cf = cs_lds<f32x4>(lds0 + bo + IMG + (k >> 1) * 512 + CS_COEF * 128 + (8 * g + 4 * (k & 1)) * 4);
-#pragma unroll
-      for (int ub = 0; ub < UB; ++ub) {
-        f32x4 e;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float x = s[k][ub][r];
-          if constexpr (MODE != CS_COL) e[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x, kq[ub], -m[ub]));
-          else if constexpr (NP == 2) e[r] = __builtin_amdgcn_exp2f(x - m[ub]) * cf[r];
-          else e[r] = __builtin_amdgcn_exp2f(x) * cf[r];
-        }
-        if constexpr (MODE != CS_COL) l[ub] += (e[0] + e[1]) + (e[2] + e[3]);
-        if constexpr (MODE == CS_COL)
-          if (hit) {
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const int32_t ln =
-                  cs_lds<int32_t>(lds0 + bo + IMG + (k >> 1) * 512 + CS_LAB * 128 + (8 * g + 4 * (k & 1) + r) * 4);
-              if (ln == (int32_t)r0 + 16 * ub + i16) e[r] = -e[r];
-            }
-          }
-        if constexpr (MODE != CS_STATS) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float a = e[2 * h], b = e[2 * h + 1];
-            if constexpr (NP == 1) pb[k >> 1][ub][0][2 * (k & 1) + h] = ib_pk(a, b);
-            else {
-              const cs_h2 hi = __builtin_bit_cast(cs_h2, __builtin_amdgcn_cvt_pkrtz(a, b));
-              const cs_h2 lo = __builtin_bit_cast(cs_h2, __builtin_amdgcn_cvt_pkrtz(a - (float)hi[0], b - (float)hi[1]));
-              pb[k >> 1][ub][0][2 * (k & 1) + h] = __builtin_bit_cast(uint32_t, hi);
-              pb[k >> 1][ub][1][2 * (k & 1) + h] = __builtin_bit_cast(uint32_t, lo);
-            }
-          }
-        }
-      }
-    }
-
-    if constexpr (MODE != CS_STATS) {
-#pragma unroll
-      for (int dt = 0; dt < NDT; ++dt) {
-        f32x4 f[UB];
-#pragma unroll
-        for (int ub = 0; ub < UB; ++ub) f[ub] = NP == 1 ? O[dt][ub] : f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int sub = 0; sub < NS; ++sub) {
-          u32x4 a[NP];
-#pragma unroll
-          for (int pl = 0; pl < NP; ++pl)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const ib_s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                  (__attribute__((address_space(3))) ib_s16x4*)(uintptr_t)(tb[dt & 7] + bo + (dt >> 3) * 256 +
-                                                                (32 * sub + 4 * h) * ROWB + pl * PLANE));
-              const u32x2 w2 = __builtin_bit_cast(u32x2, v);
-              a[pl][2 * h] = w2[0];
-              a[pl][2 * h + 1] = w2[1];
-            }
-#pragma unroll
-          for (int ub = 0; ub < UB; ++ub) {
-            if constexpr (NP == 2) {
-              f[ub] = cs_mfma<NP>(a[1], pb[sub][ub][0], f[ub]);
-              f[ub] = cs_mfma<NP>(a[0], pb[sub][ub][1], f[ub]);
-            }
-            f[ub] = cs_mfma<NP>(a[0], pb[sub][ub][0], f[ub]);
-          }
-        }
-#pragma unroll
-        for (int ub = 0; ub < UB; ++ub) O[dt][ub] = NP == 1 ? f[ub] : O[dt][ub] + f[ub];
-      }
-    }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  // The ring: at tile t's barrier its copies have landed and every wave is done with tile t - 1 (LAG: but
+  // for the product of its last group), so the copy that follows fills tile t - 1's buffer (LAG: t - 2's).
+  const bool active = r0 < p.nR;  // a wave without rows only copies
+  int buf = 0;
+  for (int64_t t = tb0; t < tb1; ++t) {
+    if (t + AHEAD > tb1) cs_wait<0>();
+    else if (MODE == CS_COL && wave == 0) cs_wait<(AHEAD - 1) * (CPT * NP + 1)>();
+    else cs_wait<(AHEAD - 1) * CPT * NP>();
     __syncthreads();
+    if (t + AHEAD < tb1) {
+      const int cb = buf + AHEAD;
+      copy(t + AHEAD, cb >= NB ? cb - NB : cb);
+    }
+    if (active)
+#pragma unroll
+      for (int gr = 0; gr < KT / (32 * SG); ++gr)
+        group(t * KT + 32 * SG * gr, buf * BUF + 32 * SG * gr * ROWB, lds0 + buf * BUF + IMG + 512 * SG * gr);
+    buf = buf + 1 == NB ? 0 : buf + 1;
+  }
+  if constexpr (LAG && MODE != CS_STATS) {
+    rescale(pend.up, pend.al);
+    if (tb0 < tb1) product(pend.bo, pend.pb, pend.al, [](int) {});
   }
 
 #pragma unroll
@@ -425,14 +585,13 @@ __global__ __launch_bounds__(64 * cs_waves(D), cs_waves(D) / 4) void cs_pass_ker
       }
       continue;
     }
-    const int64_t o = split * p.nR + q;
     if (g == 0) {
-      if constexpr (RUNMAX) p.m[o] = m[ub];
-      if constexpr (MODE != CS_COL) p.l[o] = sum;
+      if constexpr (RUNMAX) p.m[q * p.nsplit + split] = m[ub];
+      if constexpr (MODE != CS_COL) p.l[q * p.nsplit + split] = sum;
     }
     if constexpr (MODE != CS_STATS)
 #pragma unroll
-      for (int dt = 0; dt < NDT; ++dt) *reinterpret_cast<f32x4*>(p.O + o * D + 16 * dt + 4 * g) = O[dt][ub];
+      for (int dt = 0; dt < NDT; ++dt) *reinterpret_cast<f32x4*>(p.O + (split * p.nR + q) * D + 16 * dt + 4 * g) = O[dt][ub];
   }
 }
 
@@ -504,6 +663,7 @@ __global__ __launch_bounds__(256) void cs_image_kernel(CsImage p) {
     wscale = ldexpf(1.f, e);
     if ((int)blockIdx.x == p.xblocks && threadIdx.x == 0) p.scal->w_inv = ldexpf(1.f, -e);
   }
+  if (blockIdx.x == 0 && threadIdx.x < 4) p.scal->zero[threadIdx.x] = 0.f;
   const int64_t blk = is_x ? blockIdx.x : blockIdx.x - p.xblocks;
   const int64_t nblk = is_x ? p.xblocks : gridDim.x - p.xblocks;
   const int64_t rows = is_x ? p.N : p.V, rows_pad = is_x ? p.Npad : p.V;
@@ -523,12 +683,20 @@ __global__ __launch_bounds__(256) void cs_image_kernel(CsImage p) {
     if constexpr (NP == 1) {
       const uint16_t* s = (const uint16_t*)src + r * p.D + c;
       uint16_t h[4] = {0, 0, 0, 0};
-      if (r < rows)
-        for (int j = 0; j < 4; ++j)
-          if (c + j < p.D) {
-            h[j] = s[j];
-            if (is_x && lb < 0 && (h[j] & 0x7f80) == 0x7f80) h[j] = 0;
+      if (r < rows) {
+        if (vec) {
+          if (c < p.D) {
+            const u32x2 q = *reinterpret_cast<const u32x2*>(s);
+            h[0] = (uint16_t)q[0], h[1] = (uint16_t)(q[0] >> 16), h[2] = (uint16_t)q[1], h[3] = (uint16_t)(q[1] >> 16);
           }
+        } else {
+          for (int j = 0; j < 4; ++j)
+            if (c + j < p.D) h[j] = s[j];
+        }
+        if (is_x && lb < 0)
+          for (int j = 0; j < 4; ++j)
+            if ((h[j] & 0x7f80) == 0x7f80) h[j] = 0;
+      }
       *reinterpret_cast<u32x2*>(dst + r * (2 * DP) + 2 * c) =
           u32x2{h[0] | ((uint32_t)h[1] << 16), h[2] | ((uint32_t)h[3] << 16)};
     } else {
@@ -586,17 +754,20 @@ __device__ __forceinline__ float cs_ld(const void* x, int bf16, int64_t i) {
   return bf16 ? (float)((const __bf16*)x)[i] : ((const float*)x)[i];
 }
 
-// one wave per row: joins the splits, the label's logit (64-bit sums), the row's loss, its statistics
-// for the column pass and its unit gradient a q (O / l - w_y)
-template <int DP, int NP>
-__global__ __launch_bounds__(256) void cs_rows_kernel(CsRows p) {
-  constexpr int VEC = DP / 64;
-  const int lane = threadIdx.x & 63;
-  const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+// Joins the splits of a row: NWV waves per row (1: four rows per workgroup), DP / 4 lanes per split, the
+// splits dealt to the lane groups and their sums joined in a fixed order. Then the label's logit (64-bit
+// sums), the row's loss, its statistics for the column pass and its unit gradient a q (O / l - w_y).
+template <int DP, int NP, int NWV>
+__global__ __launch_bounds__(NWV == 1 ? 256 : 64 * NWV) void cs_rows_kernel(CsRows p) {
+  constexpr int LPR = DP / 4, GW = 64 / LPR, G = NWV * GW;
+  __shared__ f32x4 sh[NWV][LPR];
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+  const int64_t n = NWV == 1 ? (int64_t)blockIdx.x * 4 + wv : blockIdx.x;
+  const bool first = NWV == 1 || wv == 0;
   if (n >= p.Npad) return;
   const float kw = NP == 2 ? p.kbase * p.scal->w_inv : p.kbase;
   if (n >= p.N) {
-    if (lane == 0) {
+    if (first && lane == 0) {
       p.stat[cs_stat(n, CS_LSE2)] = INFINITY;
       p.stat[cs_stat(n, CS_COEF)] = 0.f;
       p.stat[cs_stat(n, CS_KX)] = kw;
@@ -606,14 +777,33 @@ __global__ __launch_bounds__(256) void cs_rows_kernel(CsRows p) {
     return;
   }
   const int32_t lb = p.lab[n];
+  const float* ms = p.m + n * p.nsplit;
   float M = CS_MIN;
-  for (int s = lane; s < p.nsplit; s += 64) M = fmaxf(M, p.m[s * p.N + n]);
+  for (int s = lane; s < p.nsplit; s += 64) M = fmaxf(M, ms[s]);
   M = wave_max(M);
-  double L = 0.;
-  for (int s = lane; s < p.nsplit; s += 64) {
-    const float mv = p.m[s * p.N + n];
-    L += (double)p.l[s * p.N + n] * (double)__builtin_amdgcn_exp2f(mv - M);
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  const int c = (lane % LPR) * 4;
+  if (p.dx && lb >= 0) {
+    const int64_t step = p.N * DP;
+    const float* os = p.O + n * DP + c;
+#pragma unroll 4
+    for (int s = (NWV == 1 ? 0 : wv * GW) + lane / LPR; s < p.nsplit; s += G)
+      o += *reinterpret_cast<const f32x4*>(os + s * step) * __builtin_amdgcn_exp2f(ms[s] - M);
+#pragma unroll
+    for (int k = LPR; k < 64; k <<= 1)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[j] += __shfl_xor(o[j], k, 64);
+    if constexpr (NWV > 1) {
+      if (lane < LPR) sh[wv][lane] = o;
+      __syncthreads();
+      if (wv == 0)
+        for (int k = 1; k < NWV; ++k) o += sh[k][lane % LPR];
+    }
   }
+  if (!first) return;
+  double L = 0.;
+  for (int s = lane; s < p.nsplit; s += 64)
+    L += (double)p.l[n * p.nsplit + s] * (double)__builtin_amdgcn_exp2f(ms[s] - M);
   L = wave_sum_d(L);
   // in log2 units: the other items' log sum and the label's logit
   const double o2 = L == 0. ? -INFINITY : (double)M + log2(L);
@@ -641,20 +831,11 @@ __global__ __launch_bounds__(256) void cs_rows_kernel(CsRows p) {
     reinterpret_cast<int32_t*>(p.stat)[cs_stat(n, CS_LAB)] = lb;
     p.lq[n] = (float)(o2 - lse2);
   }
-  if (!p.dx) return;
-  float o[VEC] = {};
-  if (lb >= 0) {
-    for (int s = 0; s < p.nsplit; ++s) {
-      const float f = __builtin_amdgcn_exp2f(p.m[s * p.N + n] - M);
-      const float* os = p.O + (s * p.N + n) * DP + lane * VEC;
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) o[j] += f * os[j];
-    }
-  }
+  if (!p.dx || lane >= LPR) return;
   const float il = L == 0. ? 0.f : (float)((NP == 2 ? (double)p.scal->w_inv : 1.) / L);
 #pragma unroll
-  for (int j = 0; j < VEC; ++j) {
-    const int64_t d = lane * VEC + j;
+  for (int j = 0; j < 4; ++j) {
+    const int64_t d = c + j;
     if (d >= p.D) continue;
     float v = 0.f;
     if (lb >= 0) v = L == 0. ? 0.f : a * q * (o[j] * il - cs_ld(p.w, p.bf16, (int64_t)lb * p.D + d));
@@ -671,13 +852,13 @@ __global__ __launch_bounds__(1024) void cs_total_kernel(const float* __restrict_
   __shared__ float shm[16];
   double s = 0., z = 0.;
   float cm = 0.f;
+#pragma unroll 4
   for (int64_t n = threadIdx.x; n < N; n += 1024) {
-    const int32_t lb = lab[n];
-    if (lb == -1) continue;
-    const float a = weights ? weights[n] : 1.f;
-    s += (double)a * (double)row[n];
-    z += (double)a;
-    cm = fmaxf(cm, cs_finite_abs(stat[cs_stat(n, CS_COEF)]));
+    const bool in = lab[n] != -1;
+    const float a = weights ? weights[n] : 1.f, r = row[n];
+    cm = fmaxf(cm, cs_finite_abs(stat[cs_stat(n, CS_COEF)]));  // 0 without a label
+    s += in ? (double)a * (double)r : 0.;
+    z += in ? (double)a : 0.;
   }
   s = wave_sum_d(s);
   z = wave_sum_d(z);
@@ -735,11 +916,11 @@ __global__ __launch_bounds__(256) void cs_dw_kernel(const float* __restrict__ m,
   if (v >= V) return;
   float M = CS_MIN;
   if constexpr (NP == 2)
-    for (int s = 0; s < nsplit; ++s) M = fmaxf(M, m[s * V + v]);
+    for (int s = 0; s < nsplit; ++s) M = fmaxf(M, m[v * nsplit + s]);
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
   for (int s = 0; s < nsplit; ++s) {
     const f32x4 x = *reinterpret_cast<const f32x4*>(O + (s * V + v) * DP + c);
-    if constexpr (NP == 2) o += x * __builtin_amdgcn_exp2f(m[s * V + v] - M);
+    if constexpr (NP == 2) o += x * __builtin_amdgcn_exp2f(m[v * nsplit + s] - M);
     else o += x;
   }
   float f = scale * scal->inv_z * (gscale ? *gscale : 1.f);
@@ -756,19 +937,25 @@ int cs_width(int64_t D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
 
 // Streamed ranges per resident block. Workgroups run one per CU (256 slots); a range costs its tiles
 // plus a fixed start-up and join of about 4 tiles, so the split that needs the fewest tile times wins.
-int cs_nsplit(int64_t nrb, int64_t tiles) {
+int cs_nsplit(int64_t nrb, int64_t tiles, int64_t slots) {
   int best = 1;
   int64_t best_cost = INT64_MAX;
-  for (int64_t s = 1; s <= tiles && s <= 1024 && (s == 1 || nrb * s <= 2048); ++s) {
+  for (int64_t s = 1; s <= tiles && s <= 1024 && (s == 1 || nrb * s <= 8 * slots); ++s) {
     const int64_t per = ceil_div(tiles, s);
     if (ceil_div(tiles, per) != s) continue;
-    const int64_t cost = ceil_div(nrb * s, 256) * (per + 4) + s / 16;
+    const int64_t cost = ceil_div(nrb * s, slots) * (per + 4) + s / 16;
     if (cost < best_cost) {
       best_cost = cost;
       best = (int)s;
     }
   }
   return best;
+}
+
+// workgroups per CU: 4 lb waves fit its registers
+int cs_wgs(int D, int NP, int MODE) {
+  const int n = 4 * cs_lb(D, NP, MODE) / cs_cfg(D, NP, MODE).NW;
+  return n > 1 ? n : 1;
 }
 
 struct CsShape {
@@ -778,7 +965,7 @@ struct CsShape {
   int rsplit, csplit;
   int64_t rtiles, rper, ctiles, cper, rnrb, cnrb;
 };
-CsShape cs_shape(int64_t N, int64_t V, int64_t D, int dtype) {
+CsShape cs_shape(int64_t N, int64_t V, int64_t D, int dtype, int want) {
   CsShape s;
   s.N = N;
   s.V = V;
@@ -787,14 +974,14 @@ CsShape cs_shape(int64_t N, int64_t V, int64_t D, int dtype) {
   s.NP = dtype == RS_DTYPE_F32 ? 2 : 1;
   s.es = dtype == RS_DTYPE_F32 ? 4 : 2;
   s.Npad = (N + 63) / 64 * 64;
-  s.wimage = s.NP == 2 || D != s.DP;
-  const int rows = cs_block_rows(s.DP);
-  s.rtiles = ceil_div(V, 64);
-  s.ctiles = s.Npad / 64;
-  s.rnrb = ceil_div(N, rows);
-  s.cnrb = ceil_div(V, rows);
-  s.rsplit = N ? cs_nsplit(s.rnrb, s.rtiles) : 1;
-  s.csplit = s.ctiles ? cs_nsplit(s.cnrb, s.ctiles) : 1;
+  s.wimage = s.NP == 2 || D % 8 != 0;
+  const CsCfg rc = cs_cfg(s.DP, s.NP, want & RS_CATALOG_DX ? CS_ROW : CS_STATS), cc = cs_cfg(s.DP, s.NP, CS_COL);
+  s.rtiles = ceil_div(V, rc.KT);
+  s.ctiles = s.Npad / cc.KT;
+  s.rnrb = ceil_div(N, 16 * rc.UB * rc.NW);
+  s.cnrb = ceil_div(V, 16 * cc.UB * cc.NW);
+  s.rsplit = N ? cs_nsplit(s.rnrb, s.rtiles, 256 * cs_wgs(s.DP, s.NP, CS_ROW)) : 1;
+  s.csplit = s.ctiles ? cs_nsplit(s.cnrb, s.ctiles, 256 * cs_wgs(s.DP, s.NP, CS_COL)) : 1;
   s.rper = ceil_div(s.rtiles, s.rsplit);
   s.cper = s.ctiles ? ceil_div(s.ctiles, s.csplit) : 1;
   return s;
@@ -853,7 +1040,7 @@ template <int MODE>
 void cs_launch_pass(const CsShape& s, const CsPass& p, int64_t grid, hipStream_t st) {
 #define CS_GO(WD, PL) \
   if (s.DP == WD && s.NP == PL) \
-    hipLaunchKernelGGL((cs_pass_kernel<WD, PL, MODE>), dim3((unsigned)grid), dim3(64 * cs_waves(WD)), 0, st, p);
+    hipLaunchKernelGGL((cs_pass_kernel<WD, PL, MODE>), dim3((unsigned)grid), dim3(64 * cs_cfg(WD, PL, MODE).NW), 0, st, p);
   CS_GO(64, 1) CS_GO(64, 2) CS_GO(128, 1) CS_GO(128, 2) CS_GO(256, 1) CS_GO(256, 2)
 #undef CS_GO
 }
@@ -879,12 +1066,12 @@ using namespace rs;
 
 extern "C" size_t rs_catalog_softmax_keep_bytes(int64_t N, int64_t V, int64_t D, int dtype, int want) {
   if (cs_check(N, V, D, dtype, 1.f, want, "catalog_softmax") != RS_OK) return 0;
-  return CsKeep(nullptr, 0, cs_shape(N, V, D, dtype), want).bytes;
+  return CsKeep(nullptr, 0, cs_shape(N, V, D, dtype, want), want).bytes;
 }
 
 extern "C" size_t rs_catalog_softmax_workspace_bytes(int64_t N, int64_t V, int64_t D, int dtype, int want) {
   if (cs_check(N, V, D, dtype, 1.f, want, "catalog_softmax") != RS_OK) return 0;
-  const CsShape s = cs_shape(N, V, D, dtype);
+  const CsShape s = cs_shape(N, V, D, dtype, want);
   const size_t a = CsFwdWs(nullptr, 0, s, want).bytes, b = CsBwdWs(nullptr, 0, s, want).bytes;
   return a > b ? a : b;
 }
@@ -899,7 +1086,7 @@ extern "C" int rs_catalog_softmax_fwd(const void* X, const void* W, const int64_
              "catalog_softmax_fwd: null pointer");
   RS_REQUIRE(aligned16(X) && aligned16(W) && aligned16(keep) && aligned16(workspace),
              "catalog_softmax_fwd: X, W, keep and workspace must be 16-byte aligned");
-  const CsShape s = cs_shape(N, V, D, dtype);
+  const CsShape s = cs_shape(N, V, D, dtype, want);
   const CsKeep k(keep, keep_bytes, s, want);
   const CsFwdWs w(workspace, workspace_bytes, s, want);
   if (!k.ok || !w.ok) {
@@ -927,7 +1114,13 @@ extern "C" int rs_catalog_softmax_fwd(const void* X, const void* W, const int64_
     p.nT = V;
     p.t_last = V - 1;
     p.r_plane = s.Npad * s.DP * 2;
-    p.t_plane = V * s.DP * 2;
+    p.t_plane = s.NP == 2 ? V * s.DP * 2 : 0;
+    p.r_ld = s.DP * 2;
+    p.t_ld = s.wimage ? s.DP * 2 : D * 2;
+    p.r_ch = s.DP / 8;
+    p.t_ch = (int)(p.t_ld / 16);
+    p.zero = (const char*)k.scal->zero;
+    p.nsplit = s.rsplit;
     p.tiles = s.rtiles;
     p.per = s.rper;
     p.nrb = (int)s.rnrb;
@@ -943,9 +1136,14 @@ extern "C" int rs_catalog_softmax_fwd(const void* X, const void* W, const int64_
     else cs_launch_pass<CS_STATS>(s, p, s.rnrb * s.rsplit, st);
     CsRows r{X, W, s.NP == 1, N, s.Npad, V, D, s.rsplit, w.m, w.l, w.O, k.lab, weights, k.kx, k.scal, scale, p.kbase,
              row_loss, lse, k.dx, k.stat, k.lq};
-    const dim3 gr((unsigned)(s.Npad / 4));
-#define CS_GO(WD, PL) \
-  if (s.DP == WD && s.NP == PL) hipLaunchKernelGGL((cs_rows_kernel<WD, PL>), gr, dim3(256), 0, st, r);
+    // many splits of few rows: a workgroup per row, else a wave
+    const bool wide = s.rsplit > 8;
+    const dim3 gr((unsigned)(wide ? s.Npad : s.Npad / 4));
+#define CS_GO(WD, PL)                                                                                     \
+  if (s.DP == WD && s.NP == PL) {                                                                         \
+    if (wide) hipLaunchKernelGGL((cs_rows_kernel<WD, PL, 8>), gr, dim3(512), 0, st, r);                   \
+    else hipLaunchKernelGGL((cs_rows_kernel<WD, PL, 1>), gr, dim3(256), 0, st, r);                        \
+  }
     CS_GO(64, 1) CS_GO(64, 2) CS_GO(128, 1) CS_GO(128, 2) CS_GO(256, 1) CS_GO(256, 2)
 #undef CS_GO
   }
@@ -963,7 +1161,7 @@ extern "C" int rs_catalog_softmax_bwd(const void* W, int64_t N, int64_t V, int64
   RS_REQUIRE(!dW || (want & RS_CATALOG_DW), "catalog_softmax_bwd: dW needs a forward with RS_CATALOG_DW");
   RS_REQUIRE(aligned16(W) && aligned16(keep) && aligned16(workspace) && aligned16(dX) && aligned16(dW),
              "catalog_softmax_bwd: W, keep, workspace, dX and dW must be 16-byte aligned");
-  const CsShape s = cs_shape(N, V, D, dtype);
+  const CsShape s = cs_shape(N, V, D, dtype, want);
   const CsKeep k(const_cast<void*>(keep), keep_bytes, s, want);
   const CsBwdWs w(workspace, workspace_bytes, s, want);
   if (!k.ok || !w.ok) {
@@ -983,6 +1181,12 @@ extern "C" int rs_catalog_softmax_bwd(const void* W, int64_t N, int64_t V, int64
     p.t_last = s.Npad - 1;
     p.r_plane = V * s.DP * 2;
     p.t_plane = s.Npad * s.DP * 2;
+    p.r_ld = s.wimage ? s.DP * 2 : D * 2;
+    p.t_ld = s.DP * 2;
+    p.r_ch = (int)(p.r_ld / 16);
+    p.t_ch = s.DP / 8;
+    p.zero = (const char*)k.scal->zero;
+    p.nsplit = s.csplit;
     p.tiles = s.ctiles;
     p.per = s.cper;
     p.nrb = (int)s.cnrb;
