@@ -247,14 +247,23 @@ def _typed(lib, name):
     return getattr(lib, name)
 
 
+_entries: dict = {}   # name -> typed entry point of the loaded library
+
+
+def _entry(name):
+    fn = _entries.get(name)
+    if fn is None:
+        fn = _entries[name] = _typed(load(), name)
+    return fn
+
+
 def call(name: str, *args) -> None:
     """Invoke an int-returning entry point and raise on a non-zero status."""
-    lib = load()
-    rc = _typed(lib, name)(*args)
+    rc = _entry(name)(*args)
     if rc != 0:
-        msg = lib.rs_last_error().decode(errors="replace")
+        msg = load().rs_last_error().decode(errors="replace")
         raise NativeError(f"{name} failed (status {rc}): {msg}")
 
 
 def query(name: str, *args) -> int:
-    return int(_typed(load(), name)(*args))
+    return int(_entry(name)(*args))

@@ -37,6 +37,7 @@ typedef _Float16 cs_h2 __attribute__((ext_vector_type(2)));
 
 constexpr float CS_MIN = -1e30f;     // the running maximum before any item
 constexpr float CS_PS = 15.f;        // fp16 exponentials are formed at 2^15 (below 65504)
+constexpr int CS_FEW = 64;           // rows of the few-rows path
 constexpr int CS_AMAX_BLOCKS = 512;  // partial maxima of |w|
 constexpr double CS_LOG2E = 1.4426950408889634074;
 constexpr double CS_LN2 = 0.69314718055994530942;
@@ -44,14 +45,19 @@ constexpr double CS_LN2 = 0.69314718055994530942;
 // device scalars of a call (in the kept buffer)
 struct CsScal {
   float w_inv;   // 2^-e of the catalogue's scale (fp32), 1 (bf16)
-  float c0;      // -exponent of the largest |a_n| / x-scale (fp32): keeps p a in fp16's range
   float inv_z;   // 1 / Z of the reduction
+  int32_t neg;   // a labelled row's weight is negative
   float pad;
   float zero[4];  // 16 zero bytes, for the columns past a width
 };
 
-// row statistics the column pass streams beside x: per 32 rows four arrays of 32 words
-enum { CS_LSE2 = 0, CS_COEF = 1, CS_KX = 2, CS_LAB = 3 };
+// Row statistics the column pass streams beside x, per 32 rows four arrays of 32 words: lse - log |a| in
+// log2 units (infinite where the row takes no part), the factor of its scores, its label, its weight's sign
+// bit twice (an fp16 or bf16 pair). Weights ride in the exponent: a p = sign(a) exp2(s k - (lse - log |a|)).
+// fp32: less log2 of the row's scale over CS_XREF too, the scale of rows near 1 (a small correction, so the
+// statistic keeps its low bits).
+enum { CS_LSE2 = 0, CS_KX = 1, CS_LAB = 2, CS_SIGN = 3 };
+constexpr int CS_XREF = 13;
 __host__ __device__ inline int64_t cs_stat(int64_t n, int a) { return (n >> 5) * 128 + a * 32 + (n & 31); }
 
 struct CsPass {
@@ -69,7 +75,7 @@ struct CsPass {
   const float* kx;        // row pass, fp32: 2^-e of each resident row
   const int32_t* lab;     // row pass: label of each resident row (< 0: none)
   const float* stat;      // column pass: statistics of the streamed rows
-  const float* lq;        // column pass: log2 q of the streamed rows
+  const float* lq;        // column pass: log2 (|a| q) of the streamed rows
   float *m, *l, *O;       // partials m, l [nR][split], O [split][nR][D]
   // column pass, one split: the gradient itself
   void* out;
@@ -116,29 +122,28 @@ __device__ __forceinline__ int cs_xcd(int id, int n) {
 
 enum { CS_STATS = 0, CS_ROW = 1, CS_COL = 2 };
 
-// Shape of a pass: UB 16-row subtiles of resident rows per wave, NW waves, tiles of 64 streamed rows taken
-// in groups of 32 SG rows, NB tiles in LDS; LAG: a group's second product runs beside the next group's
-// exponentials.
+// Shape of a pass: UB 16-row subtiles of resident rows per wave, NW waves, tiles of KT streamed rows taken
+// in groups of 32 SG rows, NB tiles in LDS (the copies run NB - 1 tiles ahead), WG workgroups per CU.
 #ifndef CS_V
 #define CS_V 0
 #endif
 struct CsCfg {
-  int UB, NW, KT, NB, SG;
-  bool LAG;
+  int UB, NW, KT, NB, SG, WG;
 };
 constexpr CsCfg cs_cfg(int D, int NP, int MODE) {
-  if (D == 256) return CS_V == 1 ? CsCfg{1, 8, 32, 4, 1, true} : CS_V == 2 ? CsCfg{1, 8, 32, 4, 1, false} : CsCfg{1, 8, 64, 2, 2, false};
-  if (CS_V == 1) return {2, 8, 64, 3, 1, true};
-  if (CS_V == 2) return {2, 8, 64, 3, 1, false};
-  if (CS_V == 3) return {2, 4, 64, 2, 2, false};
-  return {2, 8, 64, 2, 2, false};
+  if (D == 256 && NP == 1 && CS_V == 1) return {2, 4, 64, 4, 1, 1};
+  if (D == 256 && NP == 1 && CS_V == 2) return {1, 4, 64, 2, 2, 2};
+  if (D == 256 && NP == 1 && CS_V == 3) return {2, 4, 64, 4, 2, 1};
+  if (D == 256) return MODE == CS_COL ? CsCfg{1, 8, 32, 4, 1, 1} : CsCfg{1, 8, 64, NP == 1 ? 4 : 2, 2, 1};
+  if (NP == 1 && MODE == CS_COL) return {2, 4, 64, 2, 1, 3};
+  return {2, 8, 64, NP == 2 && D == 128 ? 4 : 8, 2, 1};
 }
 constexpr int cs_block_rows(int D, int NP, int MODE) {
   return 16 * cs_cfg(D, NP, MODE).UB * cs_cfg(D, NP, MODE).NW;
 }
 
-// waves per SIMD the registers are budgeted for
-constexpr int cs_lb(int D, int NP, int MODE) { return D == 256 && cs_cfg(D, NP, MODE).UB == 2 ? 1 : 2; }
+// waves per SIMD its registers are budgeted for
+constexpr int cs_lb(int D, int NP, int MODE) { return cs_cfg(D, NP, MODE).WG * cs_cfg(D, NP, MODE).NW / 4; }
 
 template <int N>
 __device__ __forceinline__ void cs_wait() {
@@ -161,20 +166,20 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
   const int64_t tb0 = split * p.per, tb1 = tb0 + p.per < p.tiles ? tb0 + p.per : p.tiles;
   const uint32_t lds0 = (uint32_t) reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)smem);
 
-  constexpr int SG = cs_cfg(D, NP, MODE).SG;
-  constexpr bool LAG = cs_cfg(D, NP, MODE).LAG;
-  constexpr int CPT = PLANE / (NW * 1024);    // 16-B copies per thread and plane of a tile
-  constexpr int AHEAD = LAG ? NB - 2 : NB - 1;  // tiles copied ahead (see the loop)
-  static_assert(CPT >= 1 && KT % (32 * SG) == 0 && AHEAD >= 1 && (!LAG || MODE == CS_STATS || SG == 1), "tile shape");
+  constexpr int SG = cs_cfg(D, NP, MODE).SG, GROUPS = KT / (32 * SG);
+  constexpr int CPT = PLANE / (NW * 1024);       // 16-B copies per thread and plane of a tile
+  constexpr int AHEAD = NB - 1;                  // tiles copied ahead
+  static_assert(CPT >= 1 && KT % (32 * SG) == 0 && AHEAD >= 1, "tile shape");
   // this thread's copies of the next tile; a chunk past the rows' width comes from the zeros
   const char* src[CPT];
-  int64_t src_step[CPT];
+  int32_t src_step[CPT];
 #pragma unroll
   for (int i = 0; i < CPT; ++i) {
     const int at = i * NW * 64 + tid, band = at / D;  // 16-B chunk of the image
     const int row = band * 8 + (at % 32) / 4, ch = (at % D) / 32 * 4 + ((at & 3) ^ cs_swz(band & 3));
-    src[i] = ch < p.t_ch ? p.T + (tb0 * KT + row) * p.t_ld + ch * 16 : p.zero;
-    src_step[i] = ch < p.t_ch ? KT * p.t_ld : 0;
+    const bool in = NP == 2 || ch < p.t_ch;  // fp32's image has the whole width
+    src[i] = in ? p.T + (tb0 * KT + row) * p.t_ld + ch * 16 : p.zero;
+    src_step[i] = in ? (int32_t)(KT * p.t_ld) : 0;
   }
   auto copy = [&](int64_t t, int buf) __attribute__((always_inline)) {
     const int64_t over = t * KT + KT - 1 - p.t_last;  // rows of the tile past the last one repeat it
@@ -229,7 +234,8 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
     if constexpr (MODE != CS_COL) asm volatile("" : "+v"(kq[ub]), "+v"(lab[ub]));
   }
   const float kw = p.kbase;
-  const float ps = NP == 2 ? (MODE == CS_COL ? CS_PS + p.scal->c0 : CS_PS) : 0.f;
+  const float ps = NP == 2 ? CS_PS : 0.f;
+  const bool flip = MODE == CS_COL && p.scal->neg;
 
   // row reads: A row i16 of subtile kb = row 8 (i16 / 4) + 4 kb + i16 % 4 of 32, chunk 4 c + g
   const uint32_t ab = lds0 + (i16 >> 2) * (8 * ROWB) + (i16 & 3) * 64 + (g ^ cs_swz(i16 >> 2)) * 16;
@@ -291,10 +297,9 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
       __builtin_amdgcn_sched_barrier(0);
     }
   };
-  // O += P times the group's rows, beside(dt) placed with each column tile's instructions. fp32 operands:
-  // the group's sum in fresh accumulators, then one fp32 multiply-add that also brings O to the scale P
-  // was formed at.
-  auto product = [&](uint32_t bo, const Probs& pb, const float (&al)[UB], auto&& beside) __attribute__((always_inline)) {
+  // O += P times the group's rows. fp32 operands: the group's sum in fresh accumulators, then one fp32
+  // multiply-add that also brings O to the scale P was formed at.
+  auto product = [&](uint32_t bo, const Probs& pb, const float (&al)[UB]) __attribute__((always_inline)) {
     uint32_t at[2] = {tb[0] + bo, tb[1] + bo};
     asm("" : "+v"(at[0]), "+v"(at[1]));
     constexpr int NST = SG * NDT;
@@ -331,7 +336,6 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
           O[dt][ub] = cs_mfma<NP>(a[j & 1][0], pb.w[sub][ub][0], O[dt][ub]);
         }
       }
-      if (sub == 0) beside(dt);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
@@ -353,7 +357,7 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
   auto stat_at = [&](uint32_t st, int a, int k) __attribute__((always_inline)) {
     return st + (k >> 1) * 512 + a * 128 + (8 * g + 4 * (k & 1)) * 4;
   };
-  // f(k, ub, r, whether this element is its streamed row's label, log2 q of that row)
+  // f(k, ub, r, whether this element is its streamed row's label, log2 (|a| q) of that row)
   auto each_hit = [&](int64_t n0, uint32_t st, auto&& f) __attribute__((always_inline)) {
 #pragma unroll
     for (int k = 0; k < 2 * SG; ++k)
@@ -436,11 +440,10 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
       }
     }
   };
-  // the label's element of P: -q a (its exponential is not wanted there)
+  // the label's element of P: -q |a| (its exponential is not wanted there)
   auto patch = [&](int64_t n0, uint32_t st, Probs& pb) __attribute__((always_inline)) {
     each_hit(n0, st, [&](int k, int ub, int r, bool is, float lq) __attribute__((always_inline)) {
-      const float cf = cs_lds<float>(stat_at(st, CS_COEF, k) + 4 * r);
-      const float e = -cf * __builtin_amdgcn_exp2f(NP == 2 ? lq - m[ub] : lq);
+      const float e = -__builtin_amdgcn_exp2f(NP == 2 ? lq - m[ub] : lq);
       Probs one;
       pack(one, k, ub, f32x4{e, e, e, e});
       const uint32_t mask = r & 1 ? 0xffff0000u : 0xffffu;
@@ -452,18 +455,31 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
       }
     });
   };
+  // rows of negative weight
+  auto negate = [&](uint32_t st, Probs& pb) __attribute__((always_inline)) {
+#pragma unroll
+    for (int k = 0; k < 2 * SG; ++k) {
+      const u32x4 sg = cs_lds<u32x4>(stat_at(st, CS_SIGN, k));
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int ub = 0; ub < UB; ++ub)
+#pragma unroll
+          for (int pl = 0; pl < NP; ++pl)
+            pb.w[k >> 1][ub][pl][2 * (k & 1) + h] ^= (sg[2 * h] & 0x8000u) | (sg[2 * h + 1] & 0x80000000u);
+    }
+  };
   // exponentials of part i = (subtile k, ub) of 2 SG UB
   auto exponentials = [&](int i, uint32_t st, const Scores& s, Probs& pb) __attribute__((always_inline)) {
     const int k = i / UB, ub = i % UB;
-    f32x4 cf, ls, e;
-    if constexpr (MODE == CS_COL) cf = cs_lds<f32x4>(stat_at(st, CS_COEF, k));
+    f32x4 ls, e;
     if constexpr (MODE == CS_COL && NP == 1) ls = cs_lds<f32x4>(stat_at(st, CS_LSE2, k));
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const float x = s.v[k][ub][r];
       if constexpr (MODE != CS_COL) e[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x, kq[ub], -m[ub]));
-      else if constexpr (NP == 2) e[r] = __builtin_amdgcn_exp2f(x - m[ub]) * cf[r];
-      else e[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x, kw, -ls[r])) * cf[r];
+      else if constexpr (NP == 2) e[r] = __builtin_amdgcn_exp2f(x - m[ub]);
+      else e[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x, kw, -ls[r]));
     }
     if constexpr (MODE != CS_COL) l[ub] += (e[0] + e[1]) + (e[2] + e[3]);
     if constexpr (MODE != CS_STATS) pack(pb, k, ub, e);
@@ -477,59 +493,8 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
 #pragma unroll
           for (int ub = 0; ub < UB; ++ub) O[dt][ub] *= al[ub];
   };
-  struct Pending {  // LAG: the previous group's P, not yet in O
-    Probs pb;
-    uint32_t bo = 0;
-    float al[UB];
-    bool up = false;
-  } pend;
-#pragma unroll
-  for (int ub = 0; ub < UB; ++ub) {
-    pend.al[ub] = 1.f;
-#pragma unroll
-    for (int sub = 0; sub < SG; ++sub)
-#pragma unroll
-      for (int pl = 0; pl < NP; ++pl) pend.pb.w[sub][ub][pl] = u32x4{0, 0, 0, 0};
-  }
-  auto group = [&](int64_t n0, uint32_t bo, uint32_t st) __attribute__((always_inline)) {
-    constexpr int PARTS = 2 * SG * UB;
-    float al[UB];
-    bool up, hit;
-    Scores s;
-    Probs pb;
-    scores(bo, s);
-    prepare(n0, st, s, al, up, hit);
-    if constexpr (!LAG || MODE == CS_STATS) {
-      rescale(up, al);
-#pragma unroll
-      for (int i = 0; i < PARTS; ++i) exponentials(i, st, s, pb);
-    } else {
-      rescale(pend.up, pend.al);
-      product(pend.bo, pend.pb, pend.al, [&](int dt) __attribute__((always_inline)) {
-        if (dt % (NDT / PARTS) == 0) exponentials(dt / (NDT / PARTS), st, s, pb);
-      });
-      // keeps the exponentials here: P is used in the next group only, and would sink there
-#pragma unroll
-      for (int ub = 0; ub < UB; ++ub)
-#pragma unroll
-        for (int pl = 0; pl < NP; ++pl) asm volatile("" : "+v"(pb.w[0][ub][pl]));
-    }
-    if (MODE == CS_COL && hit) {
-      asm volatile("");  // keeps the rare path a branch
-      patch(n0, st, pb);
-    }
-    if constexpr (!LAG && MODE != CS_STATS) product(bo, pb, al, [](int) {});
-    if constexpr (LAG) {
-      pend.pb = pb;
-      pend.bo = bo;
-      pend.up = up;
-#pragma unroll
-      for (int ub = 0; ub < UB; ++ub) pend.al[ub] = al[ub];
-    }
-  };
-
-  // The ring: at tile t's barrier its copies have landed and every wave is done with tile t - 1 (LAG: but
-  // for the product of its last group), so the copy that follows fills tile t - 1's buffer (LAG: t - 2's).
+  // The ring: at tile t's barrier its copies have landed and no wave reads tile t - 1 any more; the copy
+  // that follows fills tile t - 1's buffer.
   const bool active = r0 < p.nR;  // a wave without rows only copies
   int buf = 0;
   for (int64_t t = tb0; t < tb1; ++t) {
@@ -537,19 +502,31 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
     else if (MODE == CS_COL && wave == 0) cs_wait<(AHEAD - 1) * (CPT * NP + 1)>();
     else cs_wait<(AHEAD - 1) * CPT * NP>();
     __syncthreads();
-    if (t + AHEAD < tb1) {
-      const int cb = buf + AHEAD;
-      copy(t + AHEAD, cb >= NB ? cb - NB : cb);
-    }
+    if (t + AHEAD < tb1) copy(t + AHEAD, buf == 0 ? NB - 1 : buf - 1);
     if (active)
 #pragma unroll
-      for (int gr = 0; gr < KT / (32 * SG); ++gr)
-        group(t * KT + 32 * SG * gr, buf * BUF + 32 * SG * gr * ROWB, lds0 + buf * BUF + IMG + 512 * SG * gr);
+      for (int gr = 0; gr < GROUPS; ++gr) {
+        const int64_t n0 = t * KT + 32 * SG * gr;
+        const uint32_t bo = buf * BUF + 32 * SG * gr * ROWB, st = lds0 + buf * BUF + IMG + 512 * SG * gr;
+        float al[UB];
+        bool up, hit;
+        Scores s;
+        Probs pb;
+        scores(bo, s);
+        prepare(n0, st, s, al, up, hit);
+        rescale(up, al);
+#pragma unroll
+        for (int i = 0; i < 2 * SG * UB; ++i) exponentials(i, st, s, pb);
+        if constexpr (MODE == CS_COL) {
+          if (hit) {
+            asm volatile("");  // keeps the rare path a branch
+            patch(n0, st, pb);
+          }
+          if (flip) negate(st, pb);
+        }
+        if constexpr (MODE != CS_STATS) product(bo, pb, al);
+      }
     buf = buf + 1 == NB ? 0 : buf + 1;
-  }
-  if constexpr (LAG && MODE != CS_STATS) {
-    rescale(pend.up, pend.al);
-    if (tb0 < tb1) product(pend.bo, pend.pb, pend.al, [](int) {});
   }
 
 #pragma unroll
@@ -562,9 +539,9 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
     }
     if (q >= p.nR) continue;
     if (MODE == CS_COL && p.ld) {
-      // dw = O 2^m (the row scales are in the coefficients), times c g / Z
+      // dw = O 2^m (x's scales are in the exponents), times c g / Z
       float f = p.scale * p.scal->inv_z * (p.gscale ? *p.gscale : 1.f);
-      if constexpr (NP == 2) f *= __builtin_amdgcn_exp2f(m[ub]);
+      if constexpr (NP == 2) f *= __builtin_amdgcn_exp2f(m[ub] - CS_XREF);
 #pragma unroll
       for (int dt = 0; dt < (MODE == CS_STATS ? 1 : NDT); ++dt) {
         const f32x4 v = O[dt][ub] * f;
@@ -592,6 +569,119 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
     if constexpr (MODE != CS_STATS)
 #pragma unroll
       for (int dt = 0; dt < NDT; ++dt) *reinterpret_cast<f32x4*>(p.O + (split * p.nR + q) * D + 16 * dt + 4 * g) = O[dt][ub];
+  }
+}
+
+// ---- the loss alone, few fp32 rows -----------------------------------------------------------------
+// Up to 64 rows against the catalogue: its bytes are the bound, so w is read once, as it lies (an image
+// would read it twice and write it), straight into the A operand of the fp32 matrix instruction (exact
+// products; 16 items x 4 columns x 16 rows each), one step of 16 items ahead. A workgroup's four waves
+// share a range of items; their maxima and sums join in LDS.
+struct CsFew {
+  const float *x, *w;
+  const int64_t* labels;
+  int64_t N, V, D, ignore;
+  int64_t steps, per;  // steps of 64 items, per workgroup
+  float kbase;
+  int32_t* lab;
+  float *m, *l;
+};
+template <int DP, int Q>
+__global__ __launch_bounds__(256) void cs_few_kernel(CsFew p) {
+  constexpr int NC = DP / 16;
+  __shared__ float sh[2][4][16 * Q];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int g = lane >> 4, i16 = lane & 15;
+  const bool vec = p.D % 4 == 0;
+  // columns 16 c + 4 g .. of a row: element j is the k = g operand of product (c, j)
+  auto load = [&](const float* row, f32x4 (&v)[NC]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const int d = 16 * c + 4 * g;
+      v[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (vec) {
+        if (d < p.D) v[c] = *reinterpret_cast<const f32x4*>(row + d);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (d + j < p.D) v[c][j] = row[d + j];
+      }
+    }
+  };
+  f32x4 xq[Q][NC];
+  int32_t lab[Q];
+  float m[Q], l[Q];
+#pragma unroll
+  for (int q = 0; q < Q; ++q) {
+    const int64_t n = 16 * q + i16 < p.N ? 16 * q + i16 : p.N - 1;
+    load(p.x + n * p.D, xq[q]);
+    const int64_t y = p.labels[n];
+    lab[q] = y == p.ignore ? -1 : (y >= 0 && y < p.V) ? (int32_t)y : -2;
+    if (blockIdx.x == 0 && wave == 0 && g == 0 && 16 * q + i16 < p.N) p.lab[n] = lab[q];
+    if (lab[q] < 0) {  // an ignored row's finite entries only
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) xq[q][c][j] = fabsf(xq[q][c][j]) <= FLT_MAX ? xq[q][c][j] : 0.f;
+    }
+    m[q] = CS_MIN;
+    l[q] = 0.f;
+  }
+  const int64_t s0 = blockIdx.x * p.per, s1 = s0 + p.per < p.steps ? s0 + p.per : p.steps;
+  auto item = [&](int64_t step) __attribute__((always_inline)) {
+    const int64_t v = step * 64 + wave * 16 + i16;
+    return p.w + (v < p.V ? v : p.V - 1) * p.D;
+  };
+  f32x4 a[2][NC];
+  auto step = [&](int64_t t, f32x4 (&now)[NC], f32x4 (&next)[NC]) __attribute__((always_inline)) {
+    load(item(t + 1 < s1 ? t + 1 : t), next);
+    const int32_t v0 = (int32_t)(t * 64 + wave * 16 + 4 * g);  // accumulator element r is item v0 + r
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      f32x4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s = __builtin_amdgcn_mfma_f32_16x16x4f32(now[c][j], xq[q][c][j], s, 0, 0, 0);
+      s *= p.kbase;
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (v0 + r >= p.V || v0 + r == lab[q]) s[r] = -INFINITY;
+      const float x = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), m[q]);  // per lane: lanes join at the end
+      float e = l[q] * __builtin_amdgcn_exp2f(m[q] - x);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) e += __builtin_amdgcn_exp2f(s[r] - x);
+      l[q] = e;
+      m[q] = x;
+    }
+  };
+  if (s0 < s1) load(item(s0), a[0]);
+  int64_t t = s0;
+  for (; t + 1 < s1; t += 2) {
+    step(t, a[0], a[1]);
+    step(t + 1, a[1], a[0]);
+  }
+  if (t < s1) step(t, a[0], a[1]);
+#pragma unroll
+  for (int q = 0; q < Q; ++q) {
+    float x = fmaxf(m[q], __shfl_xor(m[q], 16, 64));
+    x = fmaxf(x, __shfl_xor(x, 32, 64));
+    float e = l[q] * __builtin_amdgcn_exp2f(m[q] - x);
+    e += __shfl_xor(e, 16, 64);
+    e += __shfl_xor(e, 32, 64);
+    if (g == 0) {
+      sh[0][wave][16 * q + i16] = x;
+      sh[1][wave][16 * q + i16] = e;
+    }
+  }
+  __syncthreads();
+  const int n = threadIdx.x;
+  if (n < 16 * Q && n < p.N) {
+    float x = CS_MIN, e = 0.f;
+    for (int k = 0; k < 4; ++k) x = fmaxf(x, sh[0][k][n]);
+    for (int k = 0; k < 4; ++k) e += sh[1][k][n] * __builtin_amdgcn_exp2f(sh[0][k][n] - x);
+    p.m[n * gridDim.x + blockIdx.x] = x;
+    p.l[n * gridDim.x + blockIdx.x] = e;
   }
 }
 
@@ -767,11 +857,11 @@ __global__ __launch_bounds__(NWV == 1 ? 256 : 64 * NWV) void cs_rows_kernel(CsRo
   if (n >= p.Npad) return;
   const float kw = NP == 2 ? p.kbase * p.scal->w_inv : p.kbase;
   if (n >= p.N) {
-    if (first && lane == 0) {
+    if (first && lane == 0 && p.stat) {
       p.stat[cs_stat(n, CS_LSE2)] = INFINITY;
-      p.stat[cs_stat(n, CS_COEF)] = 0.f;
       p.stat[cs_stat(n, CS_KX)] = kw;
       reinterpret_cast<int32_t*>(p.stat)[cs_stat(n, CS_LAB)] = -1;
+      reinterpret_cast<int32_t*>(p.stat)[cs_stat(n, CS_SIGN)] = 0;
       p.lq[n] = 0.f;
     }
     return;
@@ -821,15 +911,17 @@ __global__ __launch_bounds__(NWV == 1 ? 256 : 64 * NWV) void cs_rows_kernel(CsRo
   if (lane == 0) {
     p.row[n] = lb >= 0 ? soft + fmaxf(t, 0.f) : lb == -1 ? 0.f : NAN;
     p.lse[n] = (float)(lse2 * CS_LN2);
+  }
+  if (lane == 0 && p.stat) {  // a column pass follows
     const bool live = lb >= 0;
-    float coef = live ? a : 0.f;
-    if (NP == 2) coef *= p.kx[n];
+    double ca = log2((double)fabsf(a));
+    if (NP == 2) ca += log2((double)p.kx[n]) + CS_XREF;
     // NaN statistics of a labelled row reach every item's gradient, as the formula's do
-    p.stat[cs_stat(n, CS_LSE2)] = live ? (float)lse2 : INFINITY;
-    p.stat[cs_stat(n, CS_COEF)] = coef;
+    p.stat[cs_stat(n, CS_LSE2)] = live ? (float)(lse2 - ca) : INFINITY;
     p.stat[cs_stat(n, CS_KX)] = NP == 2 ? fminf(fmaxf(kw * p.kx[n], FLT_MIN), FLT_MAX) : kw;
     reinterpret_cast<int32_t*>(p.stat)[cs_stat(n, CS_LAB)] = lb;
-    p.lq[n] = (float)(o2 - lse2);
+    reinterpret_cast<uint32_t*>(p.stat)[cs_stat(n, CS_SIGN)] = live && a < 0.f ? 0x80008000u : 0u;
+    p.lq[n] = (float)(o2 - lse2 + ca);
   }
   if (!p.dx || lane >= LPR) return;
   const float il = L == 0. ? 0.f : (float)((NP == 2 ? (double)p.scal->w_inv : 1.) / L);
@@ -844,44 +936,41 @@ __global__ __launch_bounds__(NWV == 1 ? 256 : 64 * NWV) void cs_rows_kernel(CsRo
   }
 }
 
-// the loss, 1 / Z and the coefficients' exponent; one workgroup, fixed order
+// the loss, 1 / Z and whether a weight is negative; one workgroup, fixed order
 __global__ __launch_bounds__(1024) void cs_total_kernel(const float* __restrict__ row, const int32_t* __restrict__ lab,
-                                                         const float* __restrict__ weights, const float* __restrict__ stat,
-                                                         int64_t N, int mean, CsScal* scal, float* __restrict__ loss) {
+                                                         const float* __restrict__ weights, int64_t N, int mean,
+                                                         CsScal* scal, float* __restrict__ loss) {
   __shared__ double sh[2][16];
-  __shared__ float shm[16];
+  __shared__ int neg;
+  if (threadIdx.x == 0) neg = 0;
+  __syncthreads();
   double s = 0., z = 0.;
-  float cm = 0.f;
+  bool below = false;
 #pragma unroll 4
   for (int64_t n = threadIdx.x; n < N; n += 1024) {
     const bool in = lab[n] != -1;
     const float a = weights ? weights[n] : 1.f, r = row[n];
-    cm = fmaxf(cm, cs_finite_abs(stat[cs_stat(n, CS_COEF)]));  // 0 without a label
+    below |= in && a < 0.f;
     s += in ? (double)a * (double)r : 0.;
     z += in ? (double)a : 0.;
   }
+  if (below) neg = 1;
   s = wave_sum_d(s);
   z = wave_sum_d(z);
-  cm = wave_max(cm);
   if ((threadIdx.x & 63) == 0) {
     sh[0][threadIdx.x >> 6] = s;
     sh[1][threadIdx.x >> 6] = z;
-    shm[threadIdx.x >> 6] = cm;
   }
   __syncthreads();
   if (threadIdx.x == 0) {
     s = z = 0.;
-    cm = 0.f;
     for (int i = 0; i < 16; ++i) {
       s += sh[0][i];
       z += sh[1][i];
-      cm = fmaxf(cm, shm[i]);
     }
     const double inv = !mean ? 1. : z != 0. ? 1. / z : 0.;
-    int e = 0;
-    if (cm > 0.f) (void)frexpf(cm, &e);  // cm < 2^e
-    scal->c0 = (float)-e;
     scal->inv_z = (float)inv;
+    scal->neg = neg;
     *loss = (float)(s * inv);
   }
 }
@@ -924,7 +1013,7 @@ __global__ __launch_bounds__(256) void cs_dw_kernel(const float* __restrict__ m,
     else o += x;
   }
   float f = scale * scal->inv_z * (gscale ? *gscale : 1.f);
-  if constexpr (NP == 2) f *= __builtin_amdgcn_exp2f(M);
+  if constexpr (NP == 2) f *= __builtin_amdgcn_exp2f(M - CS_XREF);
   for (int j = 0; j < 4; ++j)
     if (c + j < D) {
       if (bf16) ((__bf16*)out)[v * D + c + j] = (__bf16)(o[j] * f);
@@ -935,15 +1024,18 @@ __global__ __launch_bounds__(256) void cs_dw_kernel(const float* __restrict__ m,
 // ---- host ----------------------------------------------------------------------------------------
 int cs_width(int64_t D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
 
-// Streamed ranges per resident block. Workgroups run one per CU (256 slots); a range costs its tiles
-// plus a fixed start-up and join of about 4 tiles, so the split that needs the fewest tile times wins.
-int cs_nsplit(int64_t nrb, int64_t tiles, int64_t slots) {
+// Streamed ranges per resident block: the split that costs least, of `slots` workgroups at a time, each
+// taking its tiles (5 TFLOP/s of matrix work a CU, measured) and 6 us to start and end, and the
+// partials' write and read (4 TB/s). us and bytes per us.
+int cs_nsplit(int64_t nrb, int64_t tiles, const CsCfg& c, int D, int NP, int64_t rows) {
+  const int64_t slots = 256 * c.WG;
+  const double tile = 16. * c.UB * c.NW * c.KT * D * 4 * (NP == 2 ? 3 : 1) * c.WG / 5e6;
   int best = 1;
-  int64_t best_cost = INT64_MAX;
+  double best_cost = 1e300;
   for (int64_t s = 1; s <= tiles && s <= 1024 && (s == 1 || nrb * s <= 8 * slots); ++s) {
     const int64_t per = ceil_div(tiles, s);
     if (ceil_div(tiles, per) != s) continue;
-    const int64_t cost = ceil_div(nrb * s, slots) * (per + 4) + s / 16;
+    const double cost = (double)ceil_div(nrb * s, slots) * (per * tile + 6.) + (s > 1 ? rows * s * D * 8. / 4e6 : 0.);
     if (cost < best_cost) {
       best_cost = cost;
       best = (int)s;
@@ -952,16 +1044,10 @@ int cs_nsplit(int64_t nrb, int64_t tiles, int64_t slots) {
   return best;
 }
 
-// workgroups per CU: 4 lb waves fit its registers
-int cs_wgs(int D, int NP, int MODE) {
-  const int n = 4 * cs_lb(D, NP, MODE) / cs_cfg(D, NP, MODE).NW;
-  return n > 1 ? n : 1;
-}
-
 struct CsShape {
   int64_t N, Npad, V, D;
   int DP, NP, es;
-  bool wimage;
+  bool wimage, few;
   int rsplit, csplit;
   int64_t rtiles, rper, ctiles, cper, rnrb, cnrb;
 };
@@ -980,8 +1066,15 @@ CsShape cs_shape(int64_t N, int64_t V, int64_t D, int dtype, int want) {
   s.ctiles = s.Npad / cc.KT;
   s.rnrb = ceil_div(N, 16 * rc.UB * rc.NW);
   s.cnrb = ceil_div(V, 16 * cc.UB * cc.NW);
-  s.rsplit = N ? cs_nsplit(s.rnrb, s.rtiles, 256 * cs_wgs(s.DP, s.NP, CS_ROW)) : 1;
-  s.csplit = s.ctiles ? cs_nsplit(s.cnrb, s.ctiles, 256 * cs_wgs(s.DP, s.NP, CS_COL)) : 1;
+  s.rsplit = N ? cs_nsplit(s.rnrb, s.rtiles, rc, s.DP, s.NP, N) : 1;
+  s.csplit = s.ctiles ? cs_nsplit(s.cnrb, s.ctiles, cc, s.DP, s.NP, V) : 1;
+  // few rows, loss alone, fp32: cs_few_kernel, 2048 workgroups at most
+  s.few = s.NP == 2 && want == 0 && N <= CS_FEW;
+  if (s.few && N) {
+    s.rtiles = ceil_div(V, 64);
+    s.rsplit = (int)ceil_div(s.rtiles, ceil_div(s.rtiles, 2048));
+    s.wimage = false;
+  }
   s.rper = ceil_div(s.rtiles, s.rsplit);
   s.cper = s.ctiles ? ceil_div(s.ctiles, s.csplit) : 1;
   return s;
@@ -1094,7 +1187,17 @@ extern "C" int rs_catalog_softmax_fwd(const void* X, const void* W, const int64_
     return RS_ERR_WORKSPACE;
   }
   hipStream_t st = as_stream(stream);
-  if (N > 0) {
+  const float kbase = (float)((double)scale * CS_LOG2E);
+  if (N > 0 && s.few) {
+    const CsFew f{(const float*)X, (const float*)W, labels, N, V, D, ignore_index, s.rtiles, s.rper, kbase, k.lab, w.m, w.l};
+    const int Q = (int)ceil_div(N, 16);
+#define CS_GO(WD, QQ)                                          \
+  if (s.DP == WD && (Q == QQ || (QQ == 4 && Q == 3)))          \
+    hipLaunchKernelGGL((cs_few_kernel<WD, QQ>), dim3(s.rsplit), dim3(256), 0, st, f);
+    CS_GO(64, 1) CS_GO(64, 2) CS_GO(64, 4) CS_GO(128, 1) CS_GO(128, 2) CS_GO(128, 4)
+    CS_GO(256, 1) CS_GO(256, 2) CS_GO(256, 4)
+#undef CS_GO
+  } else if (N > 0) {
     if (s.NP == 2) hipLaunchKernelGGL(cs_amax_kernel, dim3(CS_AMAX_BLOCKS), dim3(256), 0, st, (const float*)W, V * D, w.part);
     const int rpb = 256 / (s.DP / 4);
     CsImage im{X,    W,    k.ximg, k.wimg, N, s.Npad, V, D, s.Npad * s.DP * 2, V * s.DP * 2, ignore_index, labels, k.lab,
@@ -1126,7 +1229,7 @@ extern "C" int rs_catalog_softmax_fwd(const void* X, const void* W, const int64_
     p.nrb = (int)s.rnrb;
     p.scal = k.scal;
     p.scale = scale;
-    p.kbase = (float)((double)scale * CS_LOG2E);
+    p.kbase = kbase;
     p.kx = k.kx;
     p.lab = k.lab;
     p.m = w.m;
@@ -1134,8 +1237,10 @@ extern "C" int rs_catalog_softmax_fwd(const void* X, const void* W, const int64_
     p.O = w.O;
     if (want & RS_CATALOG_DX) cs_launch_pass<CS_ROW>(s, p, s.rnrb * s.rsplit, st);
     else cs_launch_pass<CS_STATS>(s, p, s.rnrb * s.rsplit, st);
-    CsRows r{X, W, s.NP == 1, N, s.Npad, V, D, s.rsplit, w.m, w.l, w.O, k.lab, weights, k.kx, k.scal, scale, p.kbase,
-             row_loss, lse, k.dx, k.stat, k.lq};
+  }
+  if (N > 0) {
+    CsRows r{X, W, s.NP == 1, N, s.Npad, V, D, s.rsplit, w.m, w.l, w.O, k.lab, weights, k.kx, k.scal, scale, kbase,
+             row_loss, lse, k.dx, want & RS_CATALOG_DW ? k.stat : nullptr, k.lq};
     // many splits of few rows: a workgroup per row, else a wave
     const bool wide = s.rsplit > 8;
     const dim3 gr((unsigned)(wide ? s.Npad : s.Npad / 4));
@@ -1147,7 +1252,7 @@ extern "C" int rs_catalog_softmax_fwd(const void* X, const void* W, const int64_
     CS_GO(64, 1) CS_GO(64, 2) CS_GO(128, 1) CS_GO(128, 2) CS_GO(256, 1) CS_GO(256, 2)
 #undef CS_GO
   }
-  hipLaunchKernelGGL(cs_total_kernel, dim3(1), dim3(1024), 0, st, row_loss, k.lab, weights, k.stat, N, mean, k.scal, loss);
+  hipLaunchKernelGGL(cs_total_kernel, dim3(1), dim3(1024), 0, st, row_loss, k.lab, weights, N, mean, k.scal, loss);
   return check_launch("catalog_softmax_fwd");
 }
 

@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 import weakref
 from typing import List, Optional, Sequence, Tuple
 
@@ -1377,6 +1378,33 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
+class _on:
+    """The device of a call's tensors as the current one for the call, and its current stream."""
+    __slots__ = ("index", "prev")
+
+    def __init__(self, t: torch.Tensor):
+        self.index = t.device.index
+        self.prev = -1
+
+    def __enter__(self):
+        cur = torch.cuda.current_device()
+        if cur != self.index:
+            self.prev = cur
+            torch.cuda.set_device(self.index)
+        return torch._C._cuda_getCurrentRawStream(self.index)
+
+    def __exit__(self, *_):
+        if self.prev >= 0:
+            torch.cuda.set_device(self.prev)
+
+
+@functools.lru_cache(maxsize=1024)
+def _catalog_bytes(N, V, D, dt, want):
+    """(keep, workspace) bytes of a catalogue softmax call (pure functions of the sizes)."""
+    return (max(query("rs_catalog_softmax_keep_bytes", N, V, D, dt, want), 256),
+            max(query("rs_catalog_softmax_workspace_bytes", N, V, D, dt, want), 256))
+
+
 class CatalogSoftmaxState:
     """What catalog_softmax_fwd hands to catalog_softmax_bwd: the operands' images, the rows'
     statistics and the unit gradient of X, in one buffer that the backward only reads."""
@@ -1417,45 +1445,51 @@ def catalog_softmax_fwd(X, W, labels, scale: float = 1.0, weights=None, ignore_i
     weights for reduction "mean" (0 without a labelled row); state is for catalog_softmax_bwd.
     want_grad: False (the loss alone, about half the work), True, or a pair (dX, dW) of bools.
     A label outside [0, V) that is not ignore_index makes its row and the loss NaN."""
-    X, W = X.detach(), W.detach()
     _catalog_check(X, W, labels, weights, scale, reduction)
     want_x, want_w = want_grad if isinstance(want_grad, (tuple, list)) else (want_grad, want_grad)
     want = (RS_CATALOG_DX if want_x else 0) | (RS_CATALOG_DW if want_w else 0)
     X, W = _aligned(X), _aligned(W)
     (N, D), V, dt = X.shape, W.shape[0], RS_DTYPES[X.dtype]
     dev = X.device
-    with torch.cuda.device(dev):
-        keep = _ws(query("rs_catalog_softmax_keep_bytes", N, V, D, dt, want), dev)
-        ws = _ws(query("rs_catalog_softmax_workspace_bytes", N, V, D, dt, want), dev)
+    keep_bytes, ws_bytes = _catalog_bytes(N, V, D, dt, want)
+    with _on(X) as stream:
+        keep = torch.empty(keep_bytes, dtype=torch.uint8, device=dev)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
         loss = torch.empty((), dtype=torch.float32, device=dev)
-        row = torch.empty((N,), dtype=torch.float32, device=dev)
-        lse = torch.empty((N,), dtype=torch.float32, device=dev)
-        call("rs_catalog_softmax_fwd", _p(X), _p(W), _p(labels), _p(weights), N, V, D, dt, float(scale),
-             int(ignore_index), int(reduction == "mean"), want, _p(loss), _p(row), _p(lse), _p(keep), keep.numel(),
-             _p(ws), ws.numel(), _stream())
-    return loss, row, lse, CatalogSoftmaxState(keep, N, V, D, X.dtype, float(scale), want)
+        row = torch.empty(N, dtype=torch.float32, device=dev)
+        lse = torch.empty(N, dtype=torch.float32, device=dev)
+        call("rs_catalog_softmax_fwd", X.data_ptr(), W.data_ptr(), labels.data_ptr(),
+             weights.data_ptr() if weights is not None else None, N, V, D, dt, scale, ignore_index,
+             reduction == "mean", want, loss.data_ptr(), row.data_ptr(), lse.data_ptr(), keep.data_ptr(), keep_bytes,
+             ws.data_ptr(), ws_bytes, stream)
+    return loss, row, lse, CatalogSoftmaxState(keep, N, V, D, X.dtype, scale, want)
 
 
 def catalog_softmax_bwd(W, state: CatalogSoftmaxState, g=None, dx: bool = True, dw: bool = True):
     """Gradients of catalog_softmax_fwd's loss -> (dX or None, dW or None) in the inputs' type. W: the
     forward's; g: dL/dloss (float32 0-dim on the device; None: 1). A forward's state may be used for
     several backwards."""
-    W = W.detach()
     _dev(W, "W", state.dtype)
-    if tuple(W.shape) != (state.V, state.D) or W.device != state.keep.device:
+    dev = state.keep.device
+    if tuple(W.shape) != (state.V, state.D) or W.device != dev:
         raise ValueError("catalog_softmax_bwd: W is not the forward's")
     if (dx and not state.want & RS_CATALOG_DX) or (dw and not state.want & RS_CATALOG_DW):
         raise ValueError("catalog_softmax_bwd: the forward was not asked for this gradient (want_grad)")
-    if g is not None and (_dev(g, "g").numel() != 1 or g.device != W.device):
+    if g is not None and (_dev(g, "g").numel() != 1 or g.device != dev):
         raise ValueError("catalog_softmax_bwd: g must be one float32 value on W's device")
-    W = _aligned(W)
-    dev, dt, want = W.device, RS_DTYPES[state.dtype], state.want
-    with torch.cuda.device(dev):
-        dX = torch.empty((state.N, state.D), dtype=state.dtype, device=dev) if dx else None
-        dW = torch.empty((state.V, state.D), dtype=state.dtype, device=dev) if dw else None
-        ws = _ws(query("rs_catalog_softmax_workspace_bytes", state.N, state.V, state.D, dt, want), dev)
-        call("rs_catalog_softmax_bwd", _p(W), state.N, state.V, state.D, dt, state.scale, want, _p(g), _p(state.keep),
-             state.keep.numel(), _p(dX), _p(dW), _p(ws), ws.numel(), _stream())
+    return _catalog_bwd(_aligned(W), state, g, dx, dw)
+
+
+def _catalog_bwd(W, state, g, dx, dw):
+    N, V, D, dt, dev = state.N, state.V, state.D, RS_DTYPES[state.dtype], state.keep.device
+    ws_bytes = _catalog_bytes(N, V, D, dt, state.want)[1]
+    with _on(W) as stream:
+        dX = torch.empty((N, D), dtype=state.dtype, device=dev) if dx else None
+        dW = torch.empty((V, D), dtype=state.dtype, device=dev) if dw else None
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+        call("rs_catalog_softmax_bwd", W.data_ptr(), N, V, D, dt, state.scale, state.want,
+             g.data_ptr() if g is not None else None, state.keep.data_ptr(), state.keep.numel(),
+             dX.data_ptr() if dx else None, dW.data_ptr() if dw else None, ws.data_ptr(), ws_bytes, stream)
     return dX, dW
 
 
@@ -1474,9 +1508,9 @@ def dropout_ticket(state: torch.Tensor) -> torch.Tensor:
     """The (seed, step) of the next mask: a copy of the state, whose step is then advanced (on the
     device: a captured step draws a new mask at each replay)."""
     _ticket_check(state, "state")
-    with torch.cuda.device(state.device):
-        ticket = torch.empty((2,), dtype=torch.int64, device=state.device)
-        call("rs_dropout_ticket", _p(state), _p(ticket), _stream())
+    with _on(state) as stream:
+        ticket = torch.empty(2, dtype=torch.int64, device=state.device)
+        call("rs_dropout_ticket", state.data_ptr(), ticket.data_ptr(), stream)
     return ticket
 
 
@@ -1484,18 +1518,21 @@ def dropout_apply(x: torch.Tensor, rate: float, ticket: torch.Tensor, out: Optio
     """x / (1 - rate) where the element's Philox word under `ticket` (seed, step) is at least
     round(rate 2^32), else 0 (rs_dropout). The gradient is the same call on it with the same ticket.
     float32 or bfloat16; out may be x."""
-    x = x.detach()
     _dev_typed(x, "x"), _ticket_check(ticket, "ticket")
     if not 0.0 <= rate < 1.0:
         raise ValueError(f"dropout: rate must lie in [0, 1), got {rate!r}")
     if ticket.device != x.device:
         raise ValueError("dropout: x and ticket must be on one device")
-    with torch.cuda.device(x.device):
+    if out is not None and (_dev(out, "out", x.dtype).shape != x.shape or out.device != x.device):
+        raise ValueError("dropout: out must match x")
+    return _dropout(x, rate, ticket, out)
+
+
+def _dropout(x, rate, ticket, out=None):
+    with _on(x) as stream:
         if out is None:
             out = torch.empty_like(x)
-        elif _dev(out, "out", x.dtype).shape != x.shape or out.device != x.device:
-            raise ValueError("dropout: out must match x")
-        call("rs_dropout", _p(x), x.numel(), RS_DTYPES[x.dtype], float(rate), _p(ticket), _p(out), _stream())
+        call("rs_dropout", x.data_ptr(), x.numel(), RS_DTYPES[x.dtype], rate, ticket.data_ptr(), out.data_ptr(), stream)
     return out
 
 
@@ -2351,7 +2388,7 @@ class CatalogSoftmaxFn(torch.autograd.Function):
         if g is None:
             return (None,) * 7
         W, = ctx.saved_tensors
-        dX, dW = catalog_softmax_bwd(W, ctx.state, g.contiguous(), ctx.needs_input_grad[0], ctx.needs_input_grad[1])
+        dX, dW = _catalog_bwd(_aligned(W), ctx.state, g.contiguous(), ctx.needs_input_grad[0], ctx.needs_input_grad[1])
         return dX, dW, None, None, None, None, None
 
 
@@ -2374,7 +2411,7 @@ class DropoutFn(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         ticket, = ctx.saved_tensors
-        return dropout_apply(dy.contiguous(), ctx.rate, ticket), None, None
+        return _dropout(dy.contiguous(), ctx.rate, ticket), None, None
 
 
 def dropout(x: torch.Tensor, rate: float, ticket: torch.Tensor) -> torch.Tensor:
