@@ -37,7 +37,6 @@ typedef _Float16 cs_h2 __attribute__((ext_vector_type(2)));
 
 constexpr float CS_MIN = -1e30f;     // the running maximum before any item
 constexpr float CS_PS = 15.f;        // fp16 exponentials are formed at 2^15 (below 65504)
-constexpr int CS_FEW = 64;           // rows of the few-rows path
 constexpr int CS_AMAX_BLOCKS = 512;  // partial maxima of |w|
 constexpr double CS_LOG2E = 1.4426950408889634074;
 constexpr double CS_LN2 = 0.69314718055994530942;
@@ -52,11 +51,11 @@ struct CsScal {
 };
 
 // Row statistics the column pass streams beside x, per 32 rows four arrays of 32 words: lse - log |a| in
-// log2 units (infinite where the row takes no part), the factor of its scores, its label, its weight's sign
-// bit twice (an fp16 or bf16 pair). Weights ride in the exponent: a p = sign(a) exp2(s k - (lse - log |a|)).
-// fp32: less log2 of the row's scale over CS_XREF too, the scale of rows near 1 (a small correction, so the
-// statistic keeps its low bits).
-enum { CS_LSE2 = 0, CS_KX = 1, CS_LAB = 2, CS_SIGN = 3 };
+// log2 units (infinite where the row takes no part), the factor of its scores, twice its label plus one for
+// a negative weight (negative: no label), log2 (|a| q). Weights ride in the exponent: a p = sign(a)
+// exp2(s k - (lse - log |a|)). fp32: less log2 of the row's scale over CS_XREF too, the scale of rows near 1
+// (a small correction, so the statistics keep their low bits).
+enum { CS_LSE2 = 0, CS_KX = 1, CS_LAB = 2, CS_LQ = 3 };
 constexpr int CS_XREF = 13;
 __host__ __device__ inline int64_t cs_stat(int64_t n, int a) { return (n >> 5) * 128 + a * 32 + (n & 31); }
 
@@ -75,7 +74,6 @@ struct CsPass {
   const float* kx;        // row pass, fp32: 2^-e of each resident row
   const int32_t* lab;     // row pass: label of each resident row (< 0: none)
   const float* stat;      // column pass: statistics of the streamed rows
-  const float* lq;        // column pass: log2 (|a| q) of the streamed rows
   float *m, *l, *O;       // partials m, l [nR][split], O [split][nR][D]
   // column pass, one split: the gradient itself
   void* out;
@@ -357,17 +355,19 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
   auto stat_at = [&](uint32_t st, int a, int k) __attribute__((always_inline)) {
     return st + (k >> 1) * 512 + a * 128 + (8 * g + 4 * (k & 1)) * 4;
   };
-  // f(k, ub, r, whether this element is its streamed row's label, log2 (|a| q) of that row)
-  auto each_hit = [&](int64_t n0, uint32_t st, auto&& f) __attribute__((always_inline)) {
+  // f(k, ub, r, whether this element is its streamed row's label, that row's statistic a)
+  auto each_hit = [&](uint32_t st, int a, auto&& f) __attribute__((always_inline)) {
 #pragma unroll
-    for (int k = 0; k < 2 * SG; ++k)
+    for (int k = 0; k < 2 * SG; ++k) {
+      const u32x4 lb = cs_lds<u32x4>(stat_at(st, CS_LAB, k));
+      const f32x4 x = cs_lds<f32x4>(stat_at(st, a, k));
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int32_t at = cs_lds<int32_t>(stat_at(st, CS_LAB, k) + 4 * r) - ((int32_t)r0 + i16);
-        const float lq = p.lq[n0 + 32 * (k >> 1) + 8 * g + 4 * (k & 1) + r];
+        const int32_t at = ((int32_t)lb[r] >> 1) - ((int32_t)r0 + i16);
 #pragma unroll
-        for (int ub = 0; ub < UB; ++ub) f(k, ub, r, at == 16 * ub, lq);
+        for (int ub = 0; ub < UB; ++ub) f(k, ub, r, at == 16 * ub, x[r]);
       }
+    }
   };
   // Before a group's exponentials (its first streamed row is n0): the label's term leaves them and the
   // running maximum is raised (up, al: what that multiplies O and l by). Both are rare, and what they
@@ -387,11 +387,31 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
         }
       }
       const int ll = lane & (32 * SG - 1);
-      const int32_t lb = cs_lds<int32_t>(st + (ll >> 5) * 512 + CS_LAB * 128 + (ll & 31) * 4);
+      const int32_t lb = cs_lds<int32_t>(st + (ll >> 5) * 512 + CS_LAB * 128 + (ll & 31) * 4) >> 1;
       hit = __any((uint32_t)(lb - (int32_t)r0) < (uint32_t)(16 * UB));
-      if (hit) each_hit(n0, st, [&](int k, int ub, int r, bool is, float lq) __attribute__((always_inline)) {
-        s.v[k][ub][r] = is ? (NP == 2 ? lq : -INFINITY) : s.v[k][ub][r];
-      });
+      // the label's element becomes |a| q, and negative below; bf16's is undone by the exponential's argument
+      if (hit) {
+        asm volatile("");  // keeps the rare path a branch
+        each_hit(st, CS_LQ, [&](int k, int ub, int r, bool is, float lq) __attribute__((always_inline)) {
+          if constexpr (NP == 2) s.v[k][ub][r] = is ? lq : s.v[k][ub][r];
+        });
+        if constexpr (NP == 1) {
+          const float ik = 1.f / kw;
+#pragma unroll
+          for (int k = 0; k < 2 * SG; ++k) {
+            const u32x4 lb4 = cs_lds<u32x4>(stat_at(st, CS_LAB, k));
+            const f32x4 lq = cs_lds<f32x4>(stat_at(st, CS_LQ, k)), ls = cs_lds<f32x4>(stat_at(st, CS_LSE2, k));
+            f32x4 x;  // a weight of zero (ls infinite) leaves nothing whatever the score
+#pragma unroll
+            for (int r = 0; r < 4; ++r) x[r] = ls[r] == INFINITY ? 0.f : (lq[r] + ls[r]) * ik;
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+              for (int ub = 0; ub < UB; ++ub)
+                s.v[k][ub][r] = ((int32_t)lb4[r] >> 1) - ((int32_t)r0 + i16) == 16 * ub ? x[r] : s.v[k][ub][r];
+          }
+        }
+      }
     } else {
       bool mine = false;
 #pragma unroll
@@ -440,33 +460,26 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
       }
     }
   };
-  // the label's element of P: -q |a| (its exponential is not wanted there)
-  auto patch = [&](int64_t n0, uint32_t st, Probs& pb) __attribute__((always_inline)) {
-    each_hit(n0, st, [&](int k, int ub, int r, bool is, float lq) __attribute__((always_inline)) {
-      const float e = -__builtin_amdgcn_exp2f(NP == 2 ? lq - m[ub] : lq);
-      Probs one;
-      pack(one, k, ub, f32x4{e, e, e, e});
-      const uint32_t mask = r & 1 ? 0xffff0000u : 0xffffu;
-      const int at = 2 * (k & 1) + (r >> 1);
+  // the label's element of P is negative
+  auto patch = [&](uint32_t st, Probs& pb) __attribute__((always_inline)) {
+    each_hit(st, CS_LAB, [&](int k, int ub, int r, bool is, float) __attribute__((always_inline)) {
+      const uint32_t sign = is ? (r & 1 ? 0x80000000u : 0x8000u) : 0u;
 #pragma unroll
-      for (int pl = 0; pl < NP; ++pl) {
-        const uint32_t w = pb.w[k >> 1][ub][pl][at];
-        pb.w[k >> 1][ub][pl][at] = is ? (w & ~mask) | (one.w[k >> 1][ub][pl][at] & mask) : w;
-      }
+      for (int pl = 0; pl < NP; ++pl) pb.w[k >> 1][ub][pl][2 * (k & 1) + (r >> 1)] ^= sign;
     });
   };
   // rows of negative weight
   auto negate = [&](uint32_t st, Probs& pb) __attribute__((always_inline)) {
 #pragma unroll
     for (int k = 0; k < 2 * SG; ++k) {
-      const u32x4 sg = cs_lds<u32x4>(stat_at(st, CS_SIGN, k));
+      const u32x4 lb = cs_lds<u32x4>(stat_at(st, CS_LAB, k));
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int ub = 0; ub < UB; ++ub)
 #pragma unroll
           for (int pl = 0; pl < NP; ++pl)
-            pb.w[k >> 1][ub][pl][2 * (k & 1) + h] ^= (sg[2 * h] & 0x8000u) | (sg[2 * h + 1] & 0x80000000u);
+            pb.w[k >> 1][ub][pl][2 * (k & 1) + h] ^= ((lb[2 * h] & 1) << 15) | ((lb[2 * h + 1] & 1) << 31);
     }
   };
   // exponentials of part i = (subtile k, ub) of 2 SG UB
@@ -520,7 +533,7 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
         if constexpr (MODE == CS_COL) {
           if (hit) {
             asm volatile("");  // keeps the rare path a branch
-            patch(n0, st, pb);
+            patch(st, pb);
           }
           if (flip) negate(st, pb);
         }
@@ -573,7 +586,7 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
 }
 
 // ---- the loss alone, few fp32 rows -----------------------------------------------------------------
-// Up to 64 rows against the catalogue: its bytes are the bound, so w is read once, as it lies (an image
+// Up to 64 rows (256-wide: 32) against the catalogue: its bytes are the bound, so w is read once, as it lies (an image
 // would read it twice and write it), straight into the A operand of the fp32 matrix instruction (exact
 // products; 16 items x 4 columns x 16 rows each), one step of 16 items ahead. A workgroup's four waves
 // share a range of items; their maxima and sums join in LDS.
@@ -581,7 +594,7 @@ struct CsFew {
   const float *x, *w;
   const int64_t* labels;
   int64_t N, V, D, ignore;
-  int64_t steps, per;  // steps of 64 items, per workgroup
+  int64_t steps;  // of 64 items, dealt to the workgroups in turn
   float kbase;
   int32_t* lab;
   float *m, *l;
@@ -592,20 +605,13 @@ __global__ __launch_bounds__(256) void cs_few_kernel(CsFew p) {
   __shared__ float sh[2][4][16 * Q];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int g = lane >> 4, i16 = lane & 15;
-  const bool vec = p.D % 4 == 0;
-  // columns 16 c + 4 g .. of a row: element j is the k = g operand of product (c, j)
+  // columns 16 c + 4 g .. of a row (D % 4 == 0): element j is the k = g operand of product (c, j)
   auto load = [&](const float* row, f32x4 (&v)[NC]) __attribute__((always_inline)) {
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       const int d = 16 * c + 4 * g;
       v[c] = f32x4{0.f, 0.f, 0.f, 0.f};
-      if (vec) {
-        if (d < p.D) v[c] = *reinterpret_cast<const f32x4*>(row + d);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (d + j < p.D) v[c][j] = row[d + j];
-      }
+      if (d < p.D) v[c] = *reinterpret_cast<const f32x4*>(row + d);
     }
   };
   f32x4 xq[Q][NC];
@@ -627,14 +633,13 @@ __global__ __launch_bounds__(256) void cs_few_kernel(CsFew p) {
     m[q] = CS_MIN;
     l[q] = 0.f;
   }
-  const int64_t s0 = blockIdx.x * p.per, s1 = s0 + p.per < p.steps ? s0 + p.per : p.steps;
   auto item = [&](int64_t step) __attribute__((always_inline)) {
     const int64_t v = step * 64 + wave * 16 + i16;
     return p.w + (v < p.V ? v : p.V - 1) * p.D;
   };
   f32x4 a[2][NC];
   auto step = [&](int64_t t, f32x4 (&now)[NC], f32x4 (&next)[NC]) __attribute__((always_inline)) {
-    load(item(t + 1 < s1 ? t + 1 : t), next);
+    load(item(t + gridDim.x < p.steps ? t + gridDim.x : t), next);
     const int32_t v0 = (int32_t)(t * 64 + wave * 16 + 4 * g);  // accumulator element r is item v0 + r
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
@@ -655,13 +660,14 @@ __global__ __launch_bounds__(256) void cs_few_kernel(CsFew p) {
       m[q] = x;
     }
   };
-  if (s0 < s1) load(item(s0), a[0]);
-  int64_t t = s0;
-  for (; t + 1 < s1; t += 2) {
+  const int64_t G = gridDim.x;
+  int64_t t = blockIdx.x;
+  load(item(t), a[0]);
+  for (; t + G < p.steps; t += 2 * G) {
     step(t, a[0], a[1]);
-    step(t + 1, a[1], a[0]);
+    step(t + G, a[1], a[0]);
   }
-  if (t < s1) step(t, a[0], a[1]);
+  if (t < p.steps) step(t, a[0], a[1]);
 #pragma unroll
   for (int q = 0; q < Q; ++q) {
     float x = fmaxf(m[q], __shfl_xor(m[q], 16, 64));
@@ -838,7 +844,7 @@ struct CsRows {
   const float* kx;
   const CsScal* scal;
   float scale, kbase;
-  float *row, *lse, *dx, *stat, *lq;
+  float *row, *lse, *dx, *stat;
 };
 __device__ __forceinline__ float cs_ld(const void* x, int bf16, int64_t i) {
   return bf16 ? (float)((const __bf16*)x)[i] : ((const float*)x)[i];
@@ -861,14 +867,14 @@ __global__ __launch_bounds__(NWV == 1 ? 256 : 64 * NWV) void cs_rows_kernel(CsRo
       p.stat[cs_stat(n, CS_LSE2)] = INFINITY;
       p.stat[cs_stat(n, CS_KX)] = kw;
       reinterpret_cast<int32_t*>(p.stat)[cs_stat(n, CS_LAB)] = -1;
-      reinterpret_cast<int32_t*>(p.stat)[cs_stat(n, CS_SIGN)] = 0;
-      p.lq[n] = 0.f;
+      p.stat[cs_stat(n, CS_LQ)] = 0.f;
     }
     return;
   }
   const int32_t lb = p.lab[n];
   const float* ms = p.m + n * p.nsplit;
   float M = CS_MIN;
+#pragma unroll 4
   for (int s = lane; s < p.nsplit; s += 64) M = fmaxf(M, ms[s]);
   M = wave_max(M);
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
@@ -892,6 +898,7 @@ __global__ __launch_bounds__(NWV == 1 ? 256 : 64 * NWV) void cs_rows_kernel(CsRo
   }
   if (!first) return;
   double L = 0.;
+#pragma unroll 4
   for (int s = lane; s < p.nsplit; s += 64)
     L += (double)p.l[n * p.nsplit + s] * (double)__builtin_amdgcn_exp2f(ms[s] - M);
   L = wave_sum_d(L);
@@ -919,9 +926,8 @@ __global__ __launch_bounds__(NWV == 1 ? 256 : 64 * NWV) void cs_rows_kernel(CsRo
     // NaN statistics of a labelled row reach every item's gradient, as the formula's do
     p.stat[cs_stat(n, CS_LSE2)] = live ? (float)(lse2 - ca) : INFINITY;
     p.stat[cs_stat(n, CS_KX)] = NP == 2 ? fminf(fmaxf(kw * p.kx[n], FLT_MIN), FLT_MAX) : kw;
-    reinterpret_cast<int32_t*>(p.stat)[cs_stat(n, CS_LAB)] = lb;
-    reinterpret_cast<uint32_t*>(p.stat)[cs_stat(n, CS_SIGN)] = live && a < 0.f ? 0x80008000u : 0u;
-    p.lq[n] = (float)(o2 - lse2 + ca);
+    reinterpret_cast<int32_t*>(p.stat)[cs_stat(n, CS_LAB)] = live ? 2 * lb + (a < 0.f) : lb;
+    p.stat[cs_stat(n, CS_LQ)] = (float)(o2 - lse2 + ca);
   }
   if (!p.dx || lane >= LPR) return;
   const float il = L == 0. ? 0.f : (float)((NP == 2 ? (double)p.scal->w_inv : 1.) / L);
@@ -1068,11 +1074,11 @@ CsShape cs_shape(int64_t N, int64_t V, int64_t D, int dtype, int want) {
   s.cnrb = ceil_div(V, 16 * cc.UB * cc.NW);
   s.rsplit = N ? cs_nsplit(s.rnrb, s.rtiles, rc, s.DP, s.NP, N) : 1;
   s.csplit = s.ctiles ? cs_nsplit(s.cnrb, s.ctiles, cc, s.DP, s.NP, V) : 1;
-  // few rows, loss alone, fp32: cs_few_kernel, 2048 workgroups at most
-  s.few = s.NP == 2 && want == 0 && N <= CS_FEW;
+  // few rows, loss alone, fp32: cs_few_kernel, three workgroups a CU
+  s.few = s.NP == 2 && want == 0 && D % 4 == 0 && N <= (s.DP == 256 ? 32 : 64);
   if (s.few && N) {
     s.rtiles = ceil_div(V, 64);
-    s.rsplit = (int)ceil_div(s.rtiles, ceil_div(s.rtiles, 2048));
+    s.rsplit = (int)(s.rtiles < 768 ? s.rtiles : 768);
     s.wimage = false;
   }
   s.rper = ceil_div(s.rtiles, s.rsplit);
@@ -1084,7 +1090,7 @@ struct CsKeep {
   CsScal* scal;
   char *ximg, *wimg;
   int32_t* lab;
-  float *kx, *stat, *lq, *dx;
+  float *kx, *stat, *dx;
   bool ok;
   size_t bytes;
   CsKeep(void* base, size_t size, const CsShape& s, int want) {
@@ -1095,7 +1101,6 @@ struct CsKeep {
     lab = c.take<int32_t>(s.Npad);
     kx = c.take<float>(s.Npad);
     stat = c.take<float>(s.Npad * 4);
-    lq = c.take<float>(s.Npad);
     dx = want & RS_CATALOG_DX ? c.take<float>((size_t)s.N * s.D) : nullptr;
     bytes = align_up(c.off, 256);
     ok = c.ok();
@@ -1189,13 +1194,13 @@ extern "C" int rs_catalog_softmax_fwd(const void* X, const void* W, const int64_
   hipStream_t st = as_stream(stream);
   const float kbase = (float)((double)scale * CS_LOG2E);
   if (N > 0 && s.few) {
-    const CsFew f{(const float*)X, (const float*)W, labels, N, V, D, ignore_index, s.rtiles, s.rper, kbase, k.lab, w.m, w.l};
+    const CsFew f{(const float*)X, (const float*)W, labels, N, V, D, ignore_index, s.rtiles, kbase, k.lab, w.m, w.l};
     const int Q = (int)ceil_div(N, 16);
 #define CS_GO(WD, QQ)                                          \
   if (s.DP == WD && (Q == QQ || (QQ == 4 && Q == 3)))          \
     hipLaunchKernelGGL((cs_few_kernel<WD, QQ>), dim3(s.rsplit), dim3(256), 0, st, f);
     CS_GO(64, 1) CS_GO(64, 2) CS_GO(64, 4) CS_GO(128, 1) CS_GO(128, 2) CS_GO(128, 4)
-    CS_GO(256, 1) CS_GO(256, 2) CS_GO(256, 4)
+    CS_GO(256, 1) CS_GO(256, 2)
 #undef CS_GO
   } else if (N > 0) {
     if (s.NP == 2) hipLaunchKernelGGL(cs_amax_kernel, dim3(CS_AMAX_BLOCKS), dim3(256), 0, st, (const float*)W, V * D, w.part);
@@ -1240,7 +1245,7 @@ extern "C" int rs_catalog_softmax_fwd(const void* X, const void* W, const int64_
   }
   if (N > 0) {
     CsRows r{X, W, s.NP == 1, N, s.Npad, V, D, s.rsplit, w.m, w.l, w.O, k.lab, weights, k.kx, k.scal, scale, kbase,
-             row_loss, lse, k.dx, want & RS_CATALOG_DW ? k.stat : nullptr, k.lq};
+             row_loss, lse, k.dx, want & RS_CATALOG_DW ? k.stat : nullptr};
     // many splits of few rows: a workgroup per row, else a wave
     const bool wide = s.rsplit > 8;
     const dim3 gr((unsigned)(wide ? s.Npad : s.Npad / 4));
@@ -1299,7 +1304,6 @@ extern "C" int rs_catalog_softmax_bwd(const void* W, int64_t N, int64_t V, int64
     p.scale = scale;
     p.kbase = (float)((double)scale * CS_LOG2E);
     p.stat = k.stat;
-    p.lq = k.lq;
     p.m = w.m;
     p.O = w.O;
     p.out = dW;

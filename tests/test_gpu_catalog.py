@@ -111,3 +111,29 @@ def test_against_float64(cuda, dtype, N, V, D):
 def test_weights_ignored_scale(cuda, dtype, reduction, N, V, D, scale):
     x, w, y, a = inputs(N, V, D, dtype, seed=7, ignored=0.4, weights=True, scale=scale)
     check(x, w, y, a, scale, reduction, g=-2.5)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("N", [1, 15, 17, 33, 64, 65])
+@pytest.mark.parametrize("V,D", [(3, 4), (64, 64), (1000, 68), (4099, 128), (700, 256)])
+def test_loss_alone(cuda, dtype, N, V, D):
+    F = pkg("functional")
+    x, w, y, a = inputs(N, V, D, dtype, seed=N + V, ignored=0.2, weights=True)
+    r = reference(x, w, y, 1.0, a, "mean")
+    t = tolerances(r, N, V, D, dtype)
+    loss, row, lse, state = F.catalog_softmax_fwd(x, w, y, 1.0, a, IGN, "mean", want_grad=False)
+    within(row, r["row"], t["row"], "row")
+    within(lse, r["lse"], t["row"], "lse")
+    assert abs(float(loss) - float(r["loss"])) <= float(t["row"].max()) + 2.0 ** -22 * abs(float(r["loss"]))
+    with pytest.raises(ValueError, match="not asked"):
+        F.catalog_softmax_bwd(w, state)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_negative_and_zero_weights_and_crowded_labels(cuda, dtype):
+    """Half the rows share three labels; weights of both signs and zero."""
+    x, w, y, _ = inputs(500, 900, 128, dtype, seed=11)
+    y[::2] = torch.tensor([5, 6, 700], device="cuda")[torch.arange(250, device="cuda") % 3]
+    a = torch.linspace(-1.0, 1.0, 500, device="cuda")
+    a[10:20] = 0.0
+    check(x, w, y, a, 1.0, "sum", g=0.5)
