@@ -857,9 +857,9 @@ template <int DP, int NP, int NWV>
 __global__ __launch_bounds__(NWV == 1 ? 256 : 64 * NWV) void cs_rows_kernel(CsRows p) {
   constexpr int LPR = DP / 4, GW = 64 / LPR, G = NWV * GW;
   __shared__ f32x4 sh[NWV][LPR];
-  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-  const int64_t n = NWV == 1 ? (int64_t)blockIdx.x * 4 + wv : blockIdx.x;
-  const bool first = NWV == 1 || wv == 0;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t n = NWV == 1 ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x;
+  const bool first = NWV == 1 || wave == 0;
   if (n >= p.Npad) return;
   const float kw = NP == 2 ? p.kbase * p.scal->w_inv : p.kbase;
   if (n >= p.N) {
@@ -873,26 +873,34 @@ __global__ __launch_bounds__(NWV == 1 ? 256 : 64 * NWV) void cs_rows_kernel(CsRo
   }
   const int32_t lb = p.lab[n];
   const float* ms = p.m + n * p.nsplit;
+  const int c = (lane % LPR) * 4;
+  const float a = p.weights ? p.weights[n] : 1.f;
+  float xv[4], wv[4];  // this lane's columns of x and of the label's item, asked for before the joins
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const bool in = lb >= 0 && c + j < p.D && first;
+    xv[j] = in ? cs_ld(p.x, p.bf16, n * p.D + c + j) : 0.f;
+    wv[j] = in ? cs_ld(p.w, p.bf16, (int64_t)lb * p.D + c + j) : 0.f;
+  }
   float M = CS_MIN;
 #pragma unroll 4
   for (int s = lane; s < p.nsplit; s += 64) M = fmaxf(M, ms[s]);
   M = wave_max(M);
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  const int c = (lane % LPR) * 4;
   if (p.dx && lb >= 0) {
     const int64_t step = p.N * DP;
     const float* os = p.O + n * DP + c;
 #pragma unroll 4
-    for (int s = (NWV == 1 ? 0 : wv * GW) + lane / LPR; s < p.nsplit; s += G)
+    for (int s = (NWV == 1 ? 0 : wave * GW) + lane / LPR; s < p.nsplit; s += G)
       o += *reinterpret_cast<const f32x4*>(os + s * step) * __builtin_amdgcn_exp2f(ms[s] - M);
 #pragma unroll
     for (int k = LPR; k < 64; k <<= 1)
 #pragma unroll
       for (int j = 0; j < 4; ++j) o[j] += __shfl_xor(o[j], k, 64);
     if constexpr (NWV > 1) {
-      if (lane < LPR) sh[wv][lane] = o;
+      if (lane < LPR) sh[wave][lane] = o;
       __syncthreads();
-      if (wv == 0)
+      if (wave == 0)
         for (int k = 1; k < NWV; ++k) o += sh[k][lane % LPR];
     }
   }
@@ -902,15 +910,18 @@ __global__ __launch_bounds__(NWV == 1 ? 256 : 64 * NWV) void cs_rows_kernel(CsRo
   for (int s = lane; s < p.nsplit; s += 64)
     L += (double)p.l[n * p.nsplit + s] * (double)__builtin_amdgcn_exp2f(ms[s] - M);
   L = wave_sum_d(L);
-  // in log2 units: the other items' log sum and the label's logit
-  const double o2 = L == 0. ? -INFINITY : (double)M + log2(L);
+  // in log2 units: the other items' log sum and the label's logit. Logarithms of fp32 mantissas (error
+  // below 2^-23), sums with the exponents in 64 bits: the 64-bit logarithm, on every row, took most of
+  // this kernel's time.
+  int le = 0;
+  const double lm = L > 0. && L < INFINITY ? frexp(L, &le) : L;
+  const double o2 = L == 0. ? -INFINITY : (double)M + le + (double)__builtin_amdgcn_logf((float)lm);
   double sy = 0.;
-  if (lb >= 0) {
-    for (int64_t d = lane; d < p.D; d += 64)
-      sy += (double)cs_ld(p.x, p.bf16, n * p.D + d) * (double)cs_ld(p.w, p.bf16, (int64_t)lb * p.D + d);
-    sy = wave_sum_d(sy) * (double)p.scale * CS_LOG2E;
-  }
-  const float a = p.weights ? p.weights[n] : 1.f;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) sy += (double)xv[j] * (double)wv[j];
+#pragma unroll
+  for (int k = LPR / 2; k > 0; k >>= 1) sy += __shfl_xor(sy, k, 64);
+  sy *= (double)p.scale * CS_LOG2E;
   const float t = (float)((o2 - sy) * CS_LN2);
   const float et = expf(-fabsf(t)), soft = log1pf(et);
   const float q = t > 0.f ? 1.f / (1.f + et) : et / (1.f + et);  // NaN stays NaN
@@ -921,8 +932,8 @@ __global__ __launch_bounds__(NWV == 1 ? 256 : 64 * NWV) void cs_rows_kernel(CsRo
   }
   if (lane == 0 && p.stat) {  // a column pass follows
     const bool live = lb >= 0;
-    double ca = log2((double)fabsf(a));
-    if (NP == 2) ca += log2((double)p.kx[n]) + CS_XREF;
+    double ca = log2f(fabsf(a));
+    if (NP == 2) ca += ilogbf(p.kx[n]) + CS_XREF;
     // NaN statistics of a labelled row reach every item's gradient, as the formula's do
     p.stat[cs_stat(n, CS_LSE2)] = live ? (float)(lse2 - ca) : INFINITY;
     p.stat[cs_stat(n, CS_KX)] = NP == 2 ? fminf(fmaxf(kw * p.kx[n], FLT_MIN), FLT_MAX) : kw;
@@ -933,12 +944,11 @@ __global__ __launch_bounds__(NWV == 1 ? 256 : 64 * NWV) void cs_rows_kernel(CsRo
   const float il = L == 0. ? 0.f : (float)((NP == 2 ? (double)p.scal->w_inv : 1.) / L);
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const int64_t d = c + j;
-    if (d >= p.D) continue;
+    if (c + j >= p.D) continue;
     float v = 0.f;
-    if (lb >= 0) v = L == 0. ? 0.f : a * q * (o[j] * il - cs_ld(p.w, p.bf16, (int64_t)lb * p.D + d));
+    if (lb >= 0) v = L == 0. ? 0.f : a * q * (o[j] * il - wv[j]);
     else if (lb == -2) v = NAN;
-    p.dx[n * p.D + d] = v;
+    p.dx[n * p.D + c + j] = v;
   }
 }
 
@@ -1038,14 +1048,16 @@ int cs_nsplit(int64_t nrb, int64_t tiles, const CsCfg& c, int D, int NP, int64_t
   const double tile = 16. * c.UB * c.NW * c.KT * D * 4 * (NP == 2 ? 3 : 1) * c.WG / 5e6;
   int best = 1;
   double best_cost = 1e300;
-  for (int64_t s = 1; s <= tiles && s <= 1024 && (s == 1 || nrb * s <= 8 * slots); ++s) {
-    const int64_t per = ceil_div(tiles, s);
-    if (ceil_div(tiles, per) != s) continue;
+  // over the distinct splits, coarsest first
+  for (int64_t per = tiles, s = 1; s <= 1024 && (s == 1 || nrb * s <= 4 * slots);) {
     const double cost = (double)ceil_div(nrb * s, slots) * (per * tile + 6.) + (s > 1 ? rows * s * D * 8. / 4e6 : 0.);
     if (cost < best_cost) {
       best_cost = cost;
       best = (int)s;
     }
+    if (per <= 1) break;
+    per = ceil_div(tiles, s + 1) < per ? ceil_div(tiles, s + 1) : per - 1;
+    s = ceil_div(tiles, per);
   }
   return best;
 }
@@ -1247,11 +1259,12 @@ extern "C" int rs_catalog_softmax_fwd(const void* X, const void* W, const int64_
     CsRows r{X, W, s.NP == 1, N, s.Npad, V, D, s.rsplit, w.m, w.l, w.O, k.lab, weights, k.kx, k.scal, scale, kbase,
              row_loss, lse, k.dx, want & RS_CATALOG_DW ? k.stat : nullptr};
     // many splits of few rows: a workgroup per row, else a wave
-    const bool wide = s.rsplit > 8;
+    const int wide = s.rsplit > 64 ? 8 : s.rsplit > 8 ? 4 : 0;
     const dim3 gr((unsigned)(wide ? s.Npad : s.Npad / 4));
 #define CS_GO(WD, PL)                                                                                     \
   if (s.DP == WD && s.NP == PL) {                                                                         \
-    if (wide) hipLaunchKernelGGL((cs_rows_kernel<WD, PL, 8>), gr, dim3(512), 0, st, r);                   \
+    if (wide == 8) hipLaunchKernelGGL((cs_rows_kernel<WD, PL, 8>), gr, dim3(512), 0, st, r);              \
+    else if (wide == 4) hipLaunchKernelGGL((cs_rows_kernel<WD, PL, 4>), gr, dim3(256), 0, st, r);         \
     else hipLaunchKernelGGL((cs_rows_kernel<WD, PL, 1>), gr, dim3(256), 0, st, r);                        \
   }
     CS_GO(64, 1) CS_GO(64, 2) CS_GO(128, 1) CS_GO(128, 2) CS_GO(256, 1) CS_GO(256, 2)
