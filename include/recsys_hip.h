@@ -808,7 +808,7 @@ int rs_l2_normalize_rows_f32(const float* x, int64_t n, int64_t D, float* out, r
 /* ---- softmax cross entropy over a whole catalogue ---------------------------------------------
  * The full-catalogue form of the retrieval loss (tfrs.tasks.Retrieval, src/models.py:116,137, whose
  * vocabulary is the batch's own items). X [N][D] rows, W [V][D] items (D <= 256; both RS_DTYPE_F32 or
- * both RS_DTYPE_BF16), labels [N] in [0, V) or ignore_index, scale c > 0, weights a [N] (nullable: 1):
+ * both RS_DTYPE_BF16), labels [N] in [0, V) or ignore_index, scale c in [2^-60, 2^60], weights a [N] (nullable: 1):
  *   s_nv = c <x_n, w_v>, lse_n = log sum_v exp s_nv, row_n = lse_n - s_n,label, loss = sum a_n row_n / Z,
  * Z = 1, or with `mean` the sum of a over the labelled rows (no labelled row: loss 0). No logits are
  * stored. An ignored row has row_loss 0, enters neither loss nor gradients (whatever its x holds) and

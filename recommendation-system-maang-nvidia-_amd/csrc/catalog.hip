@@ -106,6 +106,14 @@ __device__ __forceinline__ void cs_glds16(const char* g, uint32_t dst) {
                : "memory");
 }
 
+// 2^m, an integer exponent (for ldexp) apart from a factor of one binade: an item that no row expects has
+// an m far below the smallest number while its gradient is none of these
+__device__ __forceinline__ int cs_exp2_split(float m, float& frac) {
+  const float i = fmaxf(floorf(m), -1000.f);
+  frac = __builtin_amdgcn_exp2f(fmaxf(m, -1000.f) - i);
+  return (int)i;
+}
+
 template <typename T>
 __device__ __forceinline__ T cs_lds(uint32_t off) {
   return *reinterpret_cast<__attribute__((address_space(3))) const T*>(off);
@@ -248,11 +256,12 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
   for (int dt = 0; dt < (MODE == CS_STATS ? 1 : NDT); ++dt)
 #pragma unroll
     for (int ub = 0; ub < UB; ++ub) O[dt][ub] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float m[UB], l[UB];  // the maximum of log2 terms, less ps; this lane's sum
+  float m[UB];   // the maximum of log2 terms, less ps
+  double l[UB];  // this lane's sum (a million items' terms, one group's sum at a time)
 #pragma unroll
   for (int ub = 0; ub < UB; ++ub) {
     m[ub] = CS_MIN;
-    l[ub] = 0.f;
+    l[ub] = 0.;
   }
   struct Scores {
     f32x4 v[2 * SG][UB];  // [2 sub + kb][ub]: streamed row 32 sub + 8 g + 4 kb + r, resident row 16 ub + i16
@@ -455,7 +464,7 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
           x = fmaxf(x, m[ub]);
           al[ub] = __builtin_amdgcn_exp2f(m[ub] - x);
           m[ub] = x;
-          l[ub] *= al[ub];
+          l[ub] *= (double)al[ub];
         }
       }
     }
@@ -483,7 +492,7 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
     }
   };
   // exponentials of part i = (subtile k, ub) of 2 SG UB
-  auto exponentials = [&](int i, uint32_t st, const Scores& s, Probs& pb) __attribute__((always_inline)) {
+  auto exponentials = [&](int i, uint32_t st, const Scores& s, Probs& pb, float (&sum)[UB]) __attribute__((always_inline)) {
     const int k = i / UB, ub = i % UB;
     f32x4 ls, e;
     if constexpr (MODE == CS_COL && NP == 1) ls = cs_lds<f32x4>(stat_at(st, CS_LSE2, k));
@@ -494,7 +503,7 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
       else if constexpr (NP == 2) e[r] = __builtin_amdgcn_exp2f(x - m[ub]);
       else e[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x, kw, -ls[r]));
     }
-    if constexpr (MODE != CS_COL) l[ub] += (e[0] + e[1]) + (e[2] + e[3]);
+    if constexpr (MODE != CS_COL) sum[ub] += (e[0] + e[1]) + (e[2] + e[3]);
     if constexpr (MODE != CS_STATS) pack(pb, k, ub, e);
   };
   // O and l follow a raised maximum (bf16; with fp32 operands the product does it for O)
@@ -521,7 +530,7 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
       for (int gr = 0; gr < GROUPS; ++gr) {
         const int64_t n0 = t * KT + 32 * SG * gr;
         const uint32_t bo = buf * BUF + 32 * SG * gr * ROWB, st = lds0 + buf * BUF + IMG + 512 * SG * gr;
-        float al[UB];
+        float al[UB], sum[UB] = {};
         bool up, hit;
         Scores s;
         Probs pb;
@@ -529,7 +538,10 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
         prepare(n0, st, s, al, up, hit);
         rescale(up, al);
 #pragma unroll
-        for (int i = 0; i < 2 * SG * UB; ++i) exponentials(i, st, s, pb);
+        for (int i = 0; i < 2 * SG * UB; ++i) exponentials(i, st, s, pb, sum);
+        if constexpr (MODE != CS_COL)
+#pragma unroll
+          for (int ub = 0; ub < UB; ++ub) l[ub] += (double)sum[ub];
         if constexpr (MODE == CS_COL) {
           if (hit) {
             asm volatile("");  // keeps the rare path a branch
@@ -545,7 +557,7 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
 #pragma unroll
   for (int ub = 0; ub < UB; ++ub) {
     const int64_t q = r0 + 16 * ub + i16;
-    float sum = l[ub];
+    float sum = (float)l[ub];
     if constexpr (MODE != CS_COL) {
       sum += __shfl_xor(sum, 16, 64);
       sum += __shfl_xor(sum, 32, 64);
@@ -554,10 +566,18 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
     if (MODE == CS_COL && p.ld) {
       // dw = O 2^m (x's scales are in the exponents), times c g / Z
       float f = p.scale * p.scal->inv_z * (p.gscale ? *p.gscale : 1.f);
-      if constexpr (NP == 2) f *= __builtin_amdgcn_exp2f(m[ub] - CS_XREF);
+      int ex = 0;
+      if constexpr (NP == 2) {
+        float frac;
+        ex = cs_exp2_split(m[ub], frac) - CS_XREF;
+        f *= frac;
+      }
 #pragma unroll
       for (int dt = 0; dt < (MODE == CS_STATS ? 1 : NDT); ++dt) {
-        const f32x4 v = O[dt][ub] * f;
+        f32x4 v = O[dt][ub] * f;
+        if constexpr (NP == 2)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) v[r] = ldexpf(v[r], ex);
         const int64_t d = 16 * dt + 4 * g;
         if (p.out_bf16) {
           __bf16* o = (__bf16*)p.out + q * p.ld + d;
@@ -725,7 +745,7 @@ __device__ __forceinline__ int cs_exp(float a) {
   int e;
   (void)frexpf(a, &e);  // a in [2^(e-1), 2^e)
   const int k = 14 - e;
-  return k < -100 ? -100 : k > 100 ? 100 : k;
+  return k > 126 ? 126 : k;  // at least -114; both powers are normal numbers
 }
 
 struct CsImage {
@@ -1029,11 +1049,17 @@ __global__ __launch_bounds__(256) void cs_dw_kernel(const float* __restrict__ m,
     else o += x;
   }
   float f = scale * scal->inv_z * (gscale ? *gscale : 1.f);
-  if constexpr (NP == 2) f *= __builtin_amdgcn_exp2f(M - CS_XREF);
+  int ex = 0;
+  if constexpr (NP == 2) {
+    float frac;
+    ex = cs_exp2_split(M, frac) - CS_XREF;
+    f *= frac;
+  }
   for (int j = 0; j < 4; ++j)
     if (c + j < D) {
-      if (bf16) ((__bf16*)out)[v * D + c + j] = (__bf16)(o[j] * f);
-      else ((float*)out)[v * D + c + j] = o[j] * f;
+      const float x = NP == 2 ? ldexpf(o[j] * f, ex) : o[j] * f;
+      if (bf16) ((__bf16*)out)[v * D + c + j] = (__bf16)x;
+      else ((float*)out)[v * D + c + j] = x;
     }
 }
 
@@ -1160,7 +1186,7 @@ int cs_check(int64_t N, int64_t V, int64_t D, int dtype, float scale, int want, 
              (long long)D);
   RS_REQUIRE(N < (1ll << 30) && V < (1ll << 30), "%s: N and V must be below 2^30", what);
   RS_REQUIRE(dtype == RS_DTYPE_F32 || dtype == RS_DTYPE_BF16, "%s: unknown dtype %d", what, dtype);
-  RS_REQUIRE(scale > 0.f && scale <= FLT_MAX, "%s: scale must be positive and finite", what);
+  RS_REQUIRE(scale >= 0x1p-60f && scale <= 0x1p60f, "%s: scale must lie between 2^-60 and 2^60", what);
   RS_REQUIRE((want & ~(RS_CATALOG_DX | RS_CATALOG_DW)) == 0, "%s: unknown gradient flags %d", what, want);
   if (D > 256) {
     set_error("%s: width %lld is above 256", what, (long long)D);

@@ -1430,8 +1430,8 @@ def _catalog_check(X, W, labels, weights, scale, reduction):
         raise ValueError("catalog_softmax: an empty catalogue or width")
     if X.shape[1] > CATALOG_MAX_WIDTH:
         raise NotImplementedError(f"catalog_softmax: width {X.shape[1]} > {CATALOG_MAX_WIDTH}")
-    if not (0.0 < scale < float("inf")):
-        raise ValueError(f"catalog_softmax: scale must be positive and finite, got {scale!r}")
+    if not 2.0 ** -60 <= scale <= 2.0 ** 60:
+        raise ValueError(f"catalog_softmax: scale must lie between 2^-60 and 2^60, got {scale!r}")
     if reduction not in REDUCTIONS:
         raise ValueError(f"catalog_softmax: reduction must be one of {REDUCTIONS}, got {reduction!r}")
 
@@ -1445,6 +1445,7 @@ def catalog_softmax_fwd(X, W, labels, scale: float = 1.0, weights=None, ignore_i
     weights for reduction "mean" (0 without a labelled row); state is for catalog_softmax_bwd.
     want_grad: False (the loss alone, about half the work), True, or a pair (dX, dW) of bools.
     A label outside [0, V) that is not ignore_index makes its row and the loss NaN."""
+    scale, ignore_index = float(scale), int(ignore_index)
     _catalog_check(X, W, labels, weights, scale, reduction)
     want_x, want_w = want_grad if isinstance(want_grad, (tuple, list)) else (want_grad, want_grad)
     want = (RS_CATALOG_DX if want_x else 0) | (RS_CATALOG_DW if want_w else 0)
@@ -2394,8 +2395,11 @@ class CatalogSoftmaxFn(torch.autograd.Function):
 
 def catalog_softmax_loss(X, W, labels, scale: float = 1.0, weights=None, ignore_index: int = -100,
                          reduction: str = "sum"):
-    """(loss, row_loss) of catalog_softmax_fwd, differentiable by X and W through the loss."""
-    return CatalogSoftmaxFn.apply(X, W, labels, weights, float(scale), int(ignore_index), reduction)
+    """(loss, row_loss) of catalog_softmax_fwd, differentiable by X and W through the loss (not by the
+    weights)."""
+    if weights is not None and weights.requires_grad:
+        raise ValueError("catalog_softmax_loss: the loss is not differentiable by its weights; detach them")
+    return CatalogSoftmaxFn.apply(X, W, labels, weights, scale, ignore_index, reduction)
 
 
 class DropoutFn(torch.autograd.Function):

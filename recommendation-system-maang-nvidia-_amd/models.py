@@ -103,10 +103,37 @@ class Embedding(nn.Module):
         return EmbeddingFn.apply(ids, self.weight, self.sink)
 
 
-class Tower(nn.Module):
-    """keras.Sequential([Dense(u, 'relu') for u in dims] + [Dense(D)]) (src/models.py:76-77)."""
+class Dropout(nn.Module):
+    """keras.layers.Dropout(rate): in training, elements are dropped by a counter-based generator (seed,
+    step) kept on the device and advanced once per call, so a step captured in a graph draws a new mask
+    at each replay; no mask is stored (functional.dropout). Outside training the identity."""
 
-    def __init__(self, in_dim: int, dims: List[int], out_dim: int, seed: int = 0, device=None):
+    def __init__(self, rate: float, seed: int = 0, device=None):
+        super().__init__()
+        if not 0.0 <= rate < 1.0:
+            raise ValueError(f"dropout rate must lie in [0, 1), got {rate!r}")
+        self.rate = float(rate)
+        self.register_buffer("state", _F.dropout_state(seed, device or _default_device()))
+
+    def forward(self, x, training: Optional[bool] = None):
+        if self.rate == 0.0 or not (self.training if training is None else training):
+            return x
+        return _F.dropout(x, self.rate, _F.dropout_ticket(self.state))
+
+
+def set_dropout_seed(module: nn.Module, seed: int) -> None:
+    """Restart every Dropout under `module` at step 0 of its own stream of `seed` (data-parallel ranks
+    give each rank another seed, or their masks are the same)."""
+    for j, m in enumerate(m for m in module.modules() if isinstance(m, Dropout)):
+        m.state.copy_(torch.tensor([int(seed) + 7919 * j, 0], dtype=torch.int64))
+
+
+class Tower(nn.Module):
+    """keras.Sequential([Dense(u, 'relu') for u in dims] + [Dense(D)]) (src/models.py:76-77).
+    Build extension: dropout_rate > 0 puts a Dropout after every ReLU layer (in training)."""
+
+    def __init__(self, in_dim: int, dims: List[int], out_dim: int, seed: int = 0, device=None,
+                 dropout_rate: float = 0.0):
         super().__init__()
         layers = []
         prev = in_dim
@@ -115,9 +142,19 @@ class Tower(nn.Module):
             prev = u
         layers.append(Dense(prev, out_dim, None, seed=seed + len(dims), device=device))
         self.layers = nn.ModuleList(layers)
+        self.dropouts = (nn.ModuleList([Dropout(dropout_rate, seed=seed + 7919 * (j + 1), device=device)
+                                        for j in range(len(layers) - 1)]) if dropout_rate > 0 else None)
 
-    def forward(self, x):
-        return dense_stack(self.layers, x)
+    def drops(self, training: Optional[bool] = None) -> bool:
+        """Whether a forward draws dropout masks."""
+        return self.dropouts is not None and (self.training if training is None else training)
+
+    def forward(self, x, training: Optional[bool] = None):
+        if not self.drops(training):
+            return dense_stack(self.layers, x)
+        for layer, drop in zip(self.layers, self.dropouts):
+            x = drop(layer(x), training=True)
+        return self.layers[-1](x)
 
 
 def dense_stack(layers, x, l2: float = 0.0):
@@ -261,10 +298,11 @@ class MultiTowerModel(nn.Module):
 
     Build extension: ``user_vocab`` / ``item_vocab`` may also be an int vocabulary SIZE (tables of
     size+1 rows, integer-id inputs only) for synthetic 10M-row tables where a Python list of
-    10M strings would dominate start-up."""
+    10M strings would dominate start-up. ``tower_dropout``: dropout after the towers' ReLU layers in
+    training (catalog_loss; the reference's towers have none)."""
 
     def __init__(self, config: ModelConfig, user_vocab, item_vocab,
-                 feature_specs: Dict[str, Any], seed: int = 0, device=None):
+                 feature_specs: Dict[str, Any], seed: int = 0, device=None, tower_dropout: float = 0.0):
         super().__init__()
         device = device or _default_device()
         self.config = config
@@ -278,8 +316,11 @@ class MultiTowerModel(nn.Module):
         self.user_embedding = Embedding(nu + 1, D, seed=seed + 1, device=device)                      # :71
         self.item_lookup = None if isinstance(self.item_vocab, int) else StringLookup(self.item_vocab)  # :73
         self.item_embedding = Embedding(ni + 1, D, seed=seed + 2, device=device)                      # :74
-        self.user_tower = Tower(D, config.user_tower_dims, D, seed=seed + 10, device=device)       # :76
-        self.item_tower = Tower(D, config.item_tower_dims, D, seed=seed + 30, device=device)       # :77
+        self.tower_dropout = float(tower_dropout)
+        self.user_tower = Tower(D, config.user_tower_dims, D, seed=seed + 10, device=device,
+                                dropout_rate=self.tower_dropout)                                   # :76
+        self.item_tower = Tower(D, config.item_tower_dims, D, seed=seed + 30, device=device,
+                                dropout_rate=self.tower_dropout)                                   # :77
         set_contraction_precision(self, config.contraction_precision)
 
     @property
@@ -309,17 +350,38 @@ class MultiTowerModel(nn.Module):
             ue, ie = EmbeddingTablesFn.apply(
                 [self.user_embedding.sink, self.item_embedding.sink], 2, orders, self.user_ids(features["user_id"]),
                 self.item_ids(features["movie_id"]), self.user_embedding.weight, self.item_embedding.weight)
+            if self.user_tower.drops(training) or self.item_tower.drops(training):
+                return {"user_embedding": self.user_tower(ue, training), "item_embedding": self.item_tower(ie, training)}
             u, i = dense_stack_group([self.user_tower.layers, self.item_tower.layers], [ue, ie])
             return {"user_embedding": u, "item_embedding": i}
         if "user_id" in features:                             # :84-85
-            user_emb = self.user_tower(self.user_embedding(self.user_ids(features["user_id"])))
+            user_emb = self.user_tower(self.user_embedding(self.user_ids(features["user_id"])), training)
         if "movie_id" in features:                            # :88-89
-            item_emb = self.item_tower(self.item_embedding(self.item_ids(features["movie_id"])))
+            item_emb = self.item_tower(self.item_embedding(self.item_ids(features["movie_id"])), training)
         return {"user_embedding": user_emb, "item_embedding": item_emb}
 
+    def encode_catalog(self, training=None) -> torch.Tensor:
+        """The item tower over every row of the item table, the OOV row first: [V + 1, D]."""
+        ids = torch.arange(self.item_embedding.weight.shape[0], dtype=torch.int64, device=self.device)
+        return self.item_tower(self.item_embedding(ids), training)
+
+    def catalog_loss(self, features: Dict[str, Any], scale: float = 1.0, weights: Optional[torch.Tensor] = None,
+                     ignore_index: int = -100, reduction: str = "sum", training=None) -> torch.Tensor:
+        """The retrieval loss over the whole catalogue instead of the batch's items (Retrieval(),
+        src/models.py:116,137, has in-batch negatives only): softmax cross entropy of every user against
+        all encoded items, the row's own 'movie_id' the label (functional.catalog_softmax_loss; widths
+        up to 256). ignore_index=0 leaves rows of unknown items out."""
+        u = self.user_tower(self.user_embedding(self.user_ids(features["user_id"])), training)
+        labels = self.item_ids(features["movie_id"])
+        return _F.catalog_softmax_loss(u, self.encode_catalog(training), labels, scale, weights, ignore_index,
+                                       reduction)[0]
+
     def get_config(self):
-        return {"config": self.config.to_dict(), "user_vocab": self.user_vocab,
-                "item_vocab": self.item_vocab, "feature_specs": self.feature_specs}
+        cfg = {"config": self.config.to_dict(), "user_vocab": self.user_vocab,
+               "item_vocab": self.item_vocab, "feature_specs": self.feature_specs}
+        if self.tower_dropout > 0:
+            cfg["tower_dropout"] = self.tower_dropout
+        return cfg
 
     @classmethod
     def from_config(cls, config, **kw):

@@ -1,0 +1,96 @@
+"""The catalogue softmax and dropout where no GPU is needed: refusals before any launch, workspace
+queries, the modules' configuration."""
+import pytest
+import torch
+
+from conftest import pkg
+
+A = 4096  # a 16-byte aligned address that no call below dereferences
+
+
+def fwd(N=4, V=8, D=16, dtype=0, scale=1.0, want=3, keep=1 << 30, ws=1 << 30, x=A, w=A, labels=A):
+    pkg("_native").call("rs_catalog_softmax_fwd", x, w, labels, None, N, V, D, dtype, scale, -100, 0, want, A, A, A, A,
+                        keep, A, ws, None)
+
+
+def test_cpu_tensors_are_refused():
+    F = pkg("functional")
+    x, y = torch.zeros((4, 8)), torch.zeros(4, dtype=torch.int64)
+    with pytest.raises(RuntimeError, match="ROCm device"):
+        F.catalog_softmax_fwd(x, x, y)
+    with pytest.raises(RuntimeError, match="ROCm device"):
+        F.catalog_softmax_loss(x, x, y)
+    with pytest.raises(RuntimeError, match="ROCm device"):
+        F.dropout_apply(x, 0.5, torch.zeros(2, dtype=torch.int64))
+    with pytest.raises(RuntimeError, match="ROCm device"):
+        F.dropout_ticket(torch.zeros(2, dtype=torch.int64))
+
+
+@pytest.mark.parametrize("bad,match", [
+    (dict(N=-1), "bad sizes"), (dict(V=0), "bad sizes"), (dict(D=0), "bad sizes"), (dict(N=1 << 30), "2\\^30"),
+    (dict(V=1 << 30), "2\\^30"), (dict(D=257), "above 256"), (dict(dtype=7), "dtype"), (dict(scale=0.0), "scale"),
+    (dict(scale=float("nan")), "scale"), (dict(want=4), "flags"), (dict(x=None), "null"), (dict(w=None), "null"),
+    (dict(labels=None), "null"), (dict(x=A + 4), "aligned"), (dict(w=A + 8), "aligned"), (dict(keep=64), "keep"),
+    (dict(ws=64), "workspace")])
+def test_forward_refusals(bad, match):
+    with pytest.raises(pkg("_native").NativeError, match=match):
+        fwd(**bad)
+
+
+def test_backward_refusals():
+    N = pkg("_native")
+
+    def bwd(want=3, keep=1 << 30, ws=1 << 30, dx=A, dw=A, w=A):
+        N.call("rs_catalog_softmax_bwd", w, 4, 8, 16, 0, 1.0, want, None, A, keep, dx, dw, A, ws, None)
+
+    for bad, match in ((dict(want=2), "dX needs"), (dict(want=1), "dW needs"), (dict(w=None), "null"),
+                       (dict(dw=A + 2), "aligned"), (dict(keep=64), "keep")):
+        with pytest.raises(N.NativeError, match=match):
+            bwd(**bad)
+
+
+def test_dropout_refusals():
+    N = pkg("_native")
+    for args, match in (((A, -1, 0, 0.5, A, A), "bad size"), ((A, 8, 9, 0.5, A, A), "dtype"),
+                        ((A, 8, 0, 1.0, A, A), "rate"), ((A, 8, 0, -0.5, A, A), "rate"),
+                        ((A, 8, 0, float("nan"), A, A), "rate"), ((A, 8, 0, 1 - 2.0 ** -40, A, A), "keeps no element"),
+                        ((None, 8, 0, 0.5, A, A), "null")):
+        with pytest.raises(N.NativeError, match=match):
+            N.call("rs_dropout", *args, None)
+    N.call("rs_dropout", None, 0, 0, 0.5, None, None, None)   # nothing to do
+    with pytest.raises(N.NativeError, match="shared"):
+        N.call("rs_dropout_ticket", A, A, None)
+
+
+def test_workspace_queries():
+    q = pkg("_native").query
+    for dt in (0, 1):
+        for n, v, d in ((0, 1, 1), (1, 1, 1), (1000, 50_000, 96), (65_536, 1_000_000, 256)):
+            none = q("rs_catalog_softmax_keep_bytes", n, v, d, dt, 0)
+            both = q("rs_catalog_softmax_keep_bytes", n, v, d, dt, 3)
+            assert both >= none + 4 * n * d
+            assert q("rs_catalog_softmax_workspace_bytes", n, v, d, dt, 3) > 0
+    assert q("rs_catalog_softmax_keep_bytes", 4, 4, 300, 0, 0) == 0   # unsupported width
+
+
+def test_modules():
+    models, cfgm = pkg("models"), pkg("config")
+    for rate in (-0.1, 1.0):
+        with pytest.raises(ValueError, match="rate"):
+            models.Dropout(rate, device="cpu")
+    drop = models.Dropout(0.3, seed=4, device="cpu").eval()
+    x = torch.ones((2, 3))
+    assert drop(x) is x and drop.state.tolist() == [4, 0] and models.Dropout(0.0, device="cpu")(x) is x
+    plain = models.Tower(8, [16, 8], 4, device="cpu")
+    wet = models.Tower(8, [16, 8], 4, device="cpu", dropout_rate=0.5)
+    assert plain.dropouts is None and not plain.drops() and wet.drops() and not wet.eval().drops()
+    assert set(wet.state_dict()) - set(plain.state_dict()) == {"dropouts.0.state", "dropouts.1.state"}
+    assert len({tuple(d.state.tolist()) for d in wet.dropouts}) == 2
+    models.set_dropout_seed(wet, 9)
+    assert [d.state.tolist() for d in wet.dropouts] == [[9, 0], [9 + 7919, 0]]
+    cfg = cfgm.ModelConfig(embedding_dim=16, user_tower_dims=[8], item_tower_dims=[8])
+    enc = models.MultiTowerModel(cfg, ["a"], ["b"], {}, device="cpu")
+    assert "tower_dropout" not in enc.get_config() and enc.user_tower.dropouts is None
+    wet = models.MultiTowerModel(cfg, ["a"], ["b"], {}, device="cpu", tower_dropout=0.25)
+    again = models.MultiTowerModel.from_config(wet.get_config(), device="cpu")
+    assert again.tower_dropout == 0.25 and len(again.item_tower.dropouts) == 1
