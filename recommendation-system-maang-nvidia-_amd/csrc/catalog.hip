@@ -68,16 +68,17 @@ struct CsPass {
   int r_ch, t_ch;         // 16-byte chunks a row holds (the rest of the kernel's width reads as zero)
   const char* zero;       // 16 zero bytes
   int64_t tiles, per;     // streamed tiles, tiles per split
-  int nrb, nsplit;        // resident blocks, splits
+  int full, nsplit, nrb;  // the first `full` resident blocks are not split, the other nrb are
   const CsScal* scal;
   float scale, kbase;     // c, c log2 e
   const float* kx;        // row pass, fp32: 2^-e of each resident row
   const int32_t* lab;     // row pass: label of each resident row (< 0: none)
   const float* stat;      // column pass: statistics of the streamed rows
-  float *m, *l, *O;       // partials m, l [nR][split], O [split][nR][D]
-  // column pass, one split: the gradient itself
+  int64_t pR;             // rows of the partials: those of the split blocks (full = 0: all, split or not)
+  float *m, *l, *O;       // partials m, l [pR][split], O [split][pR][D]
+  // column pass: the gradient of the unsplit blocks
   void* out;
-  int64_t ld;             // its row length (0: partials)
+  int64_t ld;             // its row length
   int out_bf16;
   const float* gscale;
 };
@@ -137,9 +138,6 @@ struct CsCfg {
   int UB, NW, KT, NB, SG, WG;
 };
 constexpr CsCfg cs_cfg(int D, int NP, int MODE) {
-  if (D == 256 && NP == 1 && CS_V == 1) return {2, 4, 64, 4, 1, 1};
-  if (D == 256 && NP == 1 && CS_V == 2) return {1, 4, 64, 2, 2, 2};
-  if (D == 256 && NP == 1 && CS_V == 3) return {2, 4, 64, 4, 2, 1};
   if (D == 256) return MODE == CS_COL ? CsCfg{1, 8, 32, 4, 1, 1} : CsCfg{1, 8, 64, NP == 1 ? 4 : 2, 2, 1};
   if (NP == 1 && MODE == CS_COL) return {2, 4, 64, 2, 1, 3};
   return {2, 8, 64, NP == 2 && D == 128 ? 4 : 8, 2, 1};
@@ -150,6 +148,12 @@ constexpr int cs_block_rows(int D, int NP, int MODE) {
 
 // waves per SIMD its registers are budgeted for
 constexpr int cs_lb(int D, int NP, int MODE) { return cs_cfg(D, NP, MODE).WG * cs_cfg(D, NP, MODE).NW / 4; }
+
+// Steps that a product's LDS reads run ahead of its matrix instructions
+enum { CS_S, CS_P };
+constexpr int cs_ahead(int NP, int which) {
+  return NP == 2 ? 1 : which == CS_S ? 2 : 4;
+}
 
 template <int N>
 __device__ __forceinline__ void cs_wait() {
@@ -166,10 +170,12 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
   __shared__ __attribute__((aligned(1024))) char smem[NB * BUF];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4, i16 = lane & 15;
-  const int id = cs_xcd(blockIdx.x, gridDim.x);
-  const int split = id / p.nrb;
-  const int64_t r0 = (int64_t)(id % p.nrb) * cs_block_rows(D, NP, MODE) + wave * (16 * UB);
-  const int64_t tb0 = split * p.per, tb1 = tb0 + p.per < p.tiles ? tb0 + p.per : p.tiles;
+  const bool whole = (int)blockIdx.x < p.full;
+  const int id = whole ? cs_xcd(blockIdx.x, p.full) : cs_xcd(blockIdx.x - p.full, gridDim.x - p.full);
+  const int split = whole ? 0 : id / p.nrb;
+  const int64_t r0 = (int64_t)(whole ? id : p.full + id % p.nrb) * cs_block_rows(D, NP, MODE) + wave * (16 * UB);
+  const int64_t per = whole ? p.tiles : p.per;
+  const int64_t tb0 = split * per, tb1 = tb0 + per < p.tiles ? tb0 + per : p.tiles;
   const uint32_t lds0 = (uint32_t) reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)smem);
 
   constexpr int SG = cs_cfg(D, NP, MODE).SG, GROUPS = KT / (32 * SG);
@@ -274,20 +280,21 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
   auto scores = [&](uint32_t bo, Scores& s) __attribute__((always_inline)) {
     uint32_t at = ab + bo;
     asm("" : "+v"(at));  // the offsets below stay in the instructions
-    constexpr int NST = SG * NC;
-    u32x4 a[2][2][NP];
+    constexpr int NST = SG * NC, AH = cs_ahead(NP, CS_S);
+    u32x4 a[AH + 1][2][NP];
     auto read = [&](int j) __attribute__((always_inline)) {
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
         for (int pl = 0; pl < NP; ++pl)
-          a[j & 1][kb][pl] = cs_lds<u32x4>(at + (j / NC) * (32 * ROWB) + (j % NC) * 512 + kb * 256 + pl * PLANE);
+          a[j % (AH + 1)][kb][pl] = cs_lds<u32x4>(at + (j / NC) * (32 * ROWB) + (j % NC) * 512 + kb * 256 + pl * PLANE);
     };
-    read(0);
+#pragma unroll
+    for (int j = 0; j < AH && j < NST; ++j) read(j);
 #pragma unroll
     for (int j = 0; j < NST; ++j) {
       const int c = j % NC;
-      if (j + 1 < NST) read(j + 1);
+      if (j + AH < NST) read(j + AH);
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
@@ -296,10 +303,10 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
           f32x4 z = {0.f, 0.f, 0.f, 0.f};
           if (c > 0) z = o;
           if constexpr (NP == 2) {
-            z = cs_mfma<NP>(a[j & 1][kb][1], xq[ub][c][0], z);
-            z = cs_mfma<NP>(a[j & 1][kb][0], xq[ub][c][1], z);
+            z = cs_mfma<NP>(a[j % (AH + 1)][kb][1], xq[ub][c][0], z);
+            z = cs_mfma<NP>(a[j % (AH + 1)][kb][0], xq[ub][c][1], z);
           }
-          o = cs_mfma<NP>(a[j & 1][kb][0], xq[ub][c][0], z);
+          o = cs_mfma<NP>(a[j % (AH + 1)][kb][0], xq[ub][c][0], z);
         }
       __builtin_amdgcn_sched_barrier(0);
     }
@@ -309,8 +316,8 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
   auto product = [&](uint32_t bo, const Probs& pb, const float (&al)[UB]) __attribute__((always_inline)) {
     uint32_t at[2] = {tb[0] + bo, tb[1] + bo};
     asm("" : "+v"(at[0]), "+v"(at[1]));
-    constexpr int NST = SG * NDT;
-    u32x4 a[2][NP];
+    constexpr int NST = SG * NDT, AH = cs_ahead(NP, CS_P);
+    u32x4 a[AH + 1][NP];
     f32x4 f[UB];
     auto read = [&](int j) __attribute__((always_inline)) {
       const int dt = j / SG;
@@ -322,25 +329,26 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
               (__attribute__((address_space(3))) ib_s16x4*)(uintptr_t)(at[dt & 1] + (j % SG) * (32 * ROWB) +
                                                                        (dt >> 1) * 512 + h * 256 + pl * PLANE));
           const u32x2 w2 = __builtin_bit_cast(u32x2, v);
-          a[j & 1][pl][2 * h] = w2[0];
-          a[j & 1][pl][2 * h + 1] = w2[1];
+          a[j % (AH + 1)][pl][2 * h] = w2[0];
+          a[j % (AH + 1)][pl][2 * h + 1] = w2[1];
         }
     };
-    read(0);
+#pragma unroll
+    for (int j = 0; j < AH && j < NST; ++j) read(j);
 #pragma unroll
     for (int j = 0; j < NST; ++j) {
       const int dt = j / SG, sub = j % SG;
-      if (j + 1 < NST) read(j + 1);
+      if (j + AH < NST) read(j + AH);
 #pragma unroll
       for (int ub = 0; ub < UB; ++ub) {
         if constexpr (NP == 2) {
           if (sub == 0) f[ub] = f32x4{0.f, 0.f, 0.f, 0.f};
-          f[ub] = cs_mfma<NP>(a[j & 1][1], pb.w[sub][ub][0], f[ub]);
-          f[ub] = cs_mfma<NP>(a[j & 1][0], pb.w[sub][ub][1], f[ub]);
-          f[ub] = cs_mfma<NP>(a[j & 1][0], pb.w[sub][ub][0], f[ub]);
+          f[ub] = cs_mfma<NP>(a[j % (AH + 1)][1], pb.w[sub][ub][0], f[ub]);
+          f[ub] = cs_mfma<NP>(a[j % (AH + 1)][0], pb.w[sub][ub][1], f[ub]);
+          f[ub] = cs_mfma<NP>(a[j % (AH + 1)][0], pb.w[sub][ub][0], f[ub]);
           if (sub == SG - 1) O[dt][ub] = O[dt][ub] * al[ub] + f[ub];
         } else {
-          O[dt][ub] = cs_mfma<NP>(a[j & 1][0], pb.w[sub][ub][0], O[dt][ub]);
+          O[dt][ub] = cs_mfma<NP>(a[j % (AH + 1)][0], pb.w[sub][ub][0], O[dt][ub]);
         }
       }
       __builtin_amdgcn_sched_barrier(0);
@@ -563,7 +571,7 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
       sum += __shfl_xor(sum, 32, 64);
     }
     if (q >= p.nR) continue;
-    if (MODE == CS_COL && p.ld) {
+    if (MODE == CS_COL && whole) {
       // dw = O 2^m (x's scales are in the exponents), times c g / Z
       float f = p.scale * p.scal->inv_z * (p.gscale ? *p.gscale : 1.f);
       int ex = 0;
@@ -595,13 +603,14 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
       }
       continue;
     }
+    const int64_t qp = q - (int64_t)p.full * cs_block_rows(D, NP, MODE);
     if (g == 0) {
-      if constexpr (RUNMAX) p.m[q * p.nsplit + split] = m[ub];
-      if constexpr (MODE != CS_COL) p.l[q * p.nsplit + split] = sum;
+      if constexpr (RUNMAX) p.m[qp * p.nsplit + split] = m[ub];
+      if constexpr (MODE != CS_COL) p.l[qp * p.nsplit + split] = sum;
     }
     if constexpr (MODE != CS_STATS)
 #pragma unroll
-      for (int dt = 0; dt < NDT; ++dt) *reinterpret_cast<f32x4*>(p.O + (split * p.nR + q) * D + 16 * dt + 4 * g) = O[dt][ub];
+      for (int dt = 0; dt < NDT; ++dt) *reinterpret_cast<f32x4*>(p.O + (split * p.pR + qp) * D + 16 * dt + 4 * g) = O[dt][ub];
   }
 }
 
@@ -1066,24 +1075,36 @@ __global__ __launch_bounds__(256) void cs_dw_kernel(const float* __restrict__ m,
 // ---- host ----------------------------------------------------------------------------------------
 int cs_width(int64_t D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
 
-// Streamed ranges per resident block: the split that costs least, of `slots` workgroups at a time, each
-// taking its tiles (5 TFLOP/s of matrix work a CU, measured) and 6 us to start and end, and the
-// partials' write and read (4 TB/s). us and bytes per us.
-int cs_nsplit(int64_t nrb, int64_t tiles, const CsCfg& c, int D, int NP, int64_t rows) {
-  const int64_t slots = 256 * c.WG;
-  const double tile = 16. * c.UB * c.NW * c.KT * D * 4 * (NP == 2 ? 3 : 1) * c.WG / 5e6;
-  int best = 1;
+// How a pass's resident blocks are spread: `full` of them whole, each of the others split into s streamed
+// ranges, whichever costs least with `slots` workgroups at a time. A workgroup takes its tiles (5 TFLOP/s
+// of matrix work a CU, measured) and 6 us to start and end; partials are written and read (4 TB/s).
+// us, and bytes per us.
+struct CsSpread {
+  int full, s;
+  int64_t per;
+};
+CsSpread cs_spread(int64_t nrb, int64_t tiles, const CsCfg& c, int D, int NP, int64_t rows, bool col) {
+  const int64_t slots = 256 * c.WG, block = 16 * c.UB * c.NW;
+  const double tile = (double)block * c.KT * D * 4 * (NP == 2 ? 3 : 1) * c.WG / 5e6;
+  CsSpread best{0, 1, tiles};
+  if (nrb < 1 || tiles < 1) return best;
   double best_cost = 1e300;
-  // over the distinct splits, coarsest first
-  for (int64_t per = tiles, s = 1; s <= 1024 && (s == 1 || nrb * s <= 4 * slots);) {
-    const double cost = (double)ceil_div(nrb * s, slots) * (per * tile + 6.) + (s > 1 ? rows * s * D * 8. / 4e6 : 0.);
-    if (cost < best_cost) {
-      best_cost = cost;
-      best = (int)s;
+  // the column pass writes a whole block's gradient itself: whole rounds of blocks need no partials
+  for (int64_t full : {(int64_t)0, col ? nrb / slots * slots : (int64_t)0, col ? nrb : (int64_t)0}) {
+    const int64_t rest = nrb - full;
+    const double base = (double)ceil_div(full, slots) * (tiles * tile + 6.);
+    const int64_t part = rows - full * block;
+    // over the distinct splits, coarsest first
+    for (int64_t per = tiles, s = 1; s <= 1024 && (s == 1 || rest * s <= 4 * slots);) {
+      const double cost = base + (rest > 0 ? (double)ceil_div(rest * s, slots) * (per * tile + 6.) + part * s * D * 8. / 4e6 : 0.);
+      if (cost < best_cost) {
+        best_cost = cost;
+        best = CsSpread{(int)full, (int)s, per};
+      }
+      if (per <= 1 || rest < 1) break;
+      per = ceil_div(tiles, s + 1) < per ? ceil_div(tiles, s + 1) : per - 1;
+      s = ceil_div(tiles, per);
     }
-    if (per <= 1) break;
-    per = ceil_div(tiles, s + 1) < per ? ceil_div(tiles, s + 1) : per - 1;
-    s = ceil_div(tiles, per);
   }
   return best;
 }
@@ -1092,8 +1113,10 @@ struct CsShape {
   int64_t N, Npad, V, D;
   int DP, NP, es;
   bool wimage, few;
-  int rsplit, csplit;
-  int64_t rtiles, rper, ctiles, cper, rnrb, cnrb;
+  int rsplit;
+  CsSpread col;
+  int64_t rtiles, rper, ctiles, rnrb, cnrb;
+  int64_t prows;  // the column pass's rows with partials
 };
 CsShape cs_shape(int64_t N, int64_t V, int64_t D, int dtype, int want) {
   CsShape s;
@@ -1110,8 +1133,12 @@ CsShape cs_shape(int64_t N, int64_t V, int64_t D, int dtype, int want) {
   s.ctiles = s.Npad / cc.KT;
   s.rnrb = ceil_div(N, 16 * rc.UB * rc.NW);
   s.cnrb = ceil_div(V, 16 * cc.UB * cc.NW);
-  s.rsplit = N ? cs_nsplit(s.rnrb, s.rtiles, rc, s.DP, s.NP, N) : 1;
-  s.csplit = s.ctiles ? cs_nsplit(s.cnrb, s.ctiles, cc, s.DP, s.NP, V) : 1;
+  const CsSpread row = cs_spread(s.rnrb, s.rtiles, rc, s.DP, s.NP, N, false);
+  s.rsplit = row.s;
+  s.col = cs_spread(s.cnrb, s.ctiles, cc, s.DP, s.NP, V, true);
+  if (s.ctiles == 0) s.col.full = (int)s.cnrb;  // no rows: every gradient is the whole blocks' zero
+  s.prows = V - (int64_t)s.col.full * 16 * cc.UB * cc.NW;
+  if (s.prows < 0) s.prows = 0;
   // few rows, loss alone, fp32: cs_few_kernel, three workgroups a CU
   s.few = s.NP == 2 && want == 0 && D % 4 == 0 && N <= (s.DP == 256 ? 32 : 64);
   if (s.few && N) {
@@ -1120,7 +1147,6 @@ CsShape cs_shape(int64_t N, int64_t V, int64_t D, int dtype, int want) {
     s.wimage = false;
   }
   s.rper = ceil_div(s.rtiles, s.rsplit);
-  s.cper = s.ctiles ? ceil_div(s.ctiles, s.csplit) : 1;
   return s;
 }
 
@@ -1164,9 +1190,9 @@ struct CsBwdWs {
   size_t bytes;
   CsBwdWs(void* base, size_t size, const CsShape& s, int want) {
     Carve c(base, size);
-    const bool part = (want & RS_CATALOG_DW) && s.csplit > 1;
-    m = part ? c.take<float>((size_t)s.csplit * s.V) : nullptr;
-    O = part ? c.take<float>((size_t)s.csplit * s.V * s.DP) : nullptr;
+    const size_t part = want & RS_CATALOG_DW ? (size_t)s.col.s * s.prows : 0;
+    m = c.take<float>(part);
+    O = c.take<float>(part * s.DP);
     bytes = align_up(c.off, 256);
     ok = c.ok();
   }
@@ -1270,6 +1296,7 @@ extern "C" int rs_catalog_softmax_fwd(const void* X, const void* W, const int64_
     p.tiles = s.rtiles;
     p.per = s.rper;
     p.nrb = (int)s.rnrb;
+    p.pR = N;
     p.scal = k.scal;
     p.scale = scale;
     p.kbase = kbase;
@@ -1335,10 +1362,12 @@ extern "C" int rs_catalog_softmax_bwd(const void* W, int64_t N, int64_t V, int64
     p.r_ch = (int)(p.r_ld / 16);
     p.t_ch = s.DP / 8;
     p.zero = (const char*)k.scal->zero;
-    p.nsplit = s.csplit;
+    p.nsplit = s.col.s;
+    p.full = s.col.full;
+    p.pR = s.prows;
     p.tiles = s.ctiles;
-    p.per = s.cper;
-    p.nrb = (int)s.cnrb;
+    p.per = s.col.per;
+    p.nrb = (int)s.cnrb - s.col.full;
     p.scal = k.scal;
     p.scale = scale;
     p.kbase = (float)((double)scale * CS_LOG2E);
@@ -1346,16 +1375,17 @@ extern "C" int rs_catalog_softmax_bwd(const void* W, int64_t N, int64_t V, int64
     p.m = w.m;
     p.O = w.O;
     p.out = dW;
-    p.ld = s.csplit == 1 ? D : 0;
+    p.ld = D;
     p.out_bf16 = s.NP == 1;
     p.gscale = gscale;
-    cs_launch_pass<CS_COL>(s, p, s.cnrb * s.csplit, st);
-    if (s.csplit > 1) {
-      const dim3 gd((unsigned)ceil_div(V, 256 / (s.DP / 4)));
-#define CS_GO(WD, PL)                                                                                              \
+    cs_launch_pass<CS_COL>(s, p, p.full + (int64_t)p.nrb * p.nsplit, st);
+    if (s.prows > 0) {
+      void* out = (char*)dW + (V - s.prows) * D * s.es;
+      const dim3 gd((unsigned)ceil_div(s.prows, 256 / (s.DP / 4)));
+#define CS_GO(WD, PL)                                                                                                \
   if (s.DP == WD && s.NP == PL)                                                                                     \
-    hipLaunchKernelGGL((cs_dw_kernel<WD, PL>), gd, dim3(256), 0, st, w.m, w.O, s.csplit, V, D, scale, k.scal, gscale, \
-                       dW, s.NP == 1);
+    hipLaunchKernelGGL((cs_dw_kernel<WD, PL>), gd, dim3(256), 0, st, w.m, w.O, s.col.s, s.prows, D, scale, k.scal,  \
+                       gscale, out, s.NP == 1);
       CS_GO(64, 1) CS_GO(64, 2) CS_GO(128, 1) CS_GO(128, 2) CS_GO(256, 1) CS_GO(256, 2)
 #undef CS_GO
     }
