@@ -24,6 +24,12 @@
 // have a scale each; w, which the row pass sums over, has one. p is scaled against the running maximum
 // (kept in both passes) so that unlikely items keep their relative precision, and each tile's sum
 // is formed in fresh accumulators and added in fp32 (the matrix unit's long running sums lose bits).
+//
+// Bound: the matrix cores' rate at the clock their load leaves (1.9 to 2.1 GHz; 54 to 63 % of the cycles
+// busy), the exponentials' vector work beside them. 16384 x 1M x 128 bf16, a training step: 13.4 ms, 1.25
+// PFLOP/s of its 8 N V D flops (a large bf16 library product: 1.16); 8192 x 100k x 128 fp32: 2.0 ms, 420
+// TFLOP/s, three fp16 products each (a large fp32 library product: 0.154 PFLOP/s). Fewer than ~300 rows:
+// the catalogue's bytes.
 #include "split.hpp"
 
 #include <cfloat>
@@ -131,9 +137,11 @@ enum { CS_STATS = 0, CS_ROW = 1, CS_COL = 2 };
 
 // Shape of a pass: UB 16-row subtiles of resident rows per wave, NW waves, tiles of KT streamed rows taken
 // in groups of 32 SG rows, NB tiles in LDS (the copies run NB - 1 tiles ahead), WG workgroups per CU.
-#ifndef CS_V
-#define CS_V 0
-#endif
+// O, the resident rows and a group's scores fill the registers, two waves a SIMD. Groups of 64 rows form
+// half as many sums and maxima as groups of 32 (8192 x 100k x 128 fp32, row pass: 0.97 against 1.19 ms); the
+// bf16 column pass has registers for a third wave at groups of 32 (16384 x 1M x 128: 6.2 against 6.8 ms).
+// At 256 columns a wave holds 16 rows; the row pass takes groups of 64 (2999 x 30011 fp32: 252 against
+// 267 us), the column pass, with its statistics, groups of 32 (290 against 318 us).
 struct CsCfg {
   int UB, NW, KT, NB, SG, WG;
 };
@@ -149,11 +157,10 @@ constexpr int cs_block_rows(int D, int NP, int MODE) {
 // waves per SIMD its registers are budgeted for
 constexpr int cs_lb(int D, int NP, int MODE) { return cs_cfg(D, NP, MODE).WG * cs_cfg(D, NP, MODE).NW / 4; }
 
-// Steps that a product's LDS reads run ahead of its matrix instructions
+// Steps that a product's LDS reads run ahead of its matrix instructions: fp32 has three instructions a
+// step to hide them behind and no registers for more than one, bf16 one
 enum { CS_S, CS_P };
-constexpr int cs_ahead(int NP, int which) {
-  return NP == 2 ? 1 : which == CS_S ? 2 : 4;
-}
+constexpr int cs_ahead(int NP, int which) { return NP == 2 ? 1 : which == CS_S ? 2 : 4; }
 
 template <int N>
 __device__ __forceinline__ void cs_wait() {
@@ -164,7 +171,7 @@ template <int D, int NP, int MODE>
 __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) void cs_pass_kernel(CsPass p) {
   constexpr int UB = cs_cfg(D, NP, MODE).UB, NW = cs_cfg(D, NP, MODE).NW, KT = cs_cfg(D, NP, MODE).KT;
   constexpr int NB = cs_cfg(D, NP, MODE).NB;
-  constexpr int ROWB = 2 * D, PLANE = KT * ROWB, IMG = NP * PLANE, NS = KT / 32, NDT = D / 16, NC = D / 32;
+  constexpr int ROWB = 2 * D, PLANE = KT * ROWB, IMG = NP * PLANE, NDT = D / 16, NC = D / 32;
   constexpr int STAT = MODE == CS_COL ? KT * 16 : 0, BUF = IMG + STAT;
   constexpr bool RUNMAX = MODE != CS_COL || NP == 2;
   __shared__ __attribute__((aligned(1024))) char smem[NB * BUF];
@@ -276,7 +283,7 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
     u32x4 w[SG][UB][NP];  // the second product's B operand: k = 8 g + j of sub, j < 4 from kb = 0
   };
 
-  // S of the group's streamed rows at LDS byte bo; the next k step's rows are read ahead of this one's products
+  // S of the group's streamed rows at LDS byte bo, one step = 32 columns of 32 rows
   auto scores = [&](uint32_t bo, Scores& s) __attribute__((always_inline)) {
     uint32_t at = ab + bo;
     asm("" : "+v"(at));  // the offsets below stay in the instructions
@@ -372,17 +379,17 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
   auto stat_at = [&](uint32_t st, int a, int k) __attribute__((always_inline)) {
     return st + (k >> 1) * 512 + a * 128 + (8 * g + 4 * (k & 1)) * 4;
   };
-  // f(k, ub, r, whether this element is its streamed row's label, that row's statistic a)
-  auto each_hit = [&](uint32_t st, int a, auto&& f) __attribute__((always_inline)) {
+  // f(k, ub, r, whether this element is its streamed row's label, x(k)[r])
+  auto each_hit = [&](uint32_t st, auto&& x, auto&& f) __attribute__((always_inline)) {
 #pragma unroll
     for (int k = 0; k < 2 * SG; ++k) {
       const u32x4 lb = cs_lds<u32x4>(stat_at(st, CS_LAB, k));
-      const f32x4 x = cs_lds<f32x4>(stat_at(st, a, k));
+      const f32x4 xk = x(k);
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int32_t at = ((int32_t)lb[r] >> 1) - ((int32_t)r0 + i16);
 #pragma unroll
-        for (int ub = 0; ub < UB; ++ub) f(k, ub, r, at == 16 * ub, x[r]);
+        for (int ub = 0; ub < UB; ++ub) f(k, ub, r, at == 16 * ub, xk[r]);
       }
     }
   };
@@ -406,28 +413,25 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
       const int ll = lane & (32 * SG - 1);
       const int32_t lb = cs_lds<int32_t>(st + (ll >> 5) * 512 + CS_LAB * 128 + (ll & 31) * 4) >> 1;
       hit = __any((uint32_t)(lb - (int32_t)r0) < (uint32_t)(16 * UB));
-      // the label's element becomes |a| q, and negative below; bf16's is undone by the exponential's argument
+      // the label's element is to become |a| q (its sign follows in `patch`): fp32's scores are log2 p here;
+      // a bf16 score is the one whose exponential is |a| q, unless the row's weight is zero (ls infinite),
+      // which leaves nothing whatever the score
       if (hit) {
         asm volatile("");  // keeps the rare path a branch
-        each_hit(st, CS_LQ, [&](int k, int ub, int r, bool is, float lq) __attribute__((always_inline)) {
-          if constexpr (NP == 2) s.v[k][ub][r] = is ? lq : s.v[k][ub][r];
-        });
-        if constexpr (NP == 1) {
-          const float ik = 1.f / kw;
+        each_hit(
+            st,
+            [&](int k) __attribute__((always_inline)) {
+              f32x4 x = cs_lds<f32x4>(stat_at(st, CS_LQ, k));
+              if constexpr (NP == 1) {
+                const f32x4 ls = cs_lds<f32x4>(stat_at(st, CS_LSE2, k));
 #pragma unroll
-          for (int k = 0; k < 2 * SG; ++k) {
-            const u32x4 lb4 = cs_lds<u32x4>(stat_at(st, CS_LAB, k));
-            const f32x4 lq = cs_lds<f32x4>(stat_at(st, CS_LQ, k)), ls = cs_lds<f32x4>(stat_at(st, CS_LSE2, k));
-            f32x4 x;  // a weight of zero (ls infinite) leaves nothing whatever the score
-#pragma unroll
-            for (int r = 0; r < 4; ++r) x[r] = ls[r] == INFINITY ? 0.f : (lq[r] + ls[r]) * ik;
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-#pragma unroll
-              for (int ub = 0; ub < UB; ++ub)
-                s.v[k][ub][r] = ((int32_t)lb4[r] >> 1) - ((int32_t)r0 + i16) == 16 * ub ? x[r] : s.v[k][ub][r];
-          }
-        }
+                for (int r = 0; r < 4; ++r) x[r] = ls[r] == INFINITY ? 0.f : (x[r] + ls[r]) * (1.f / kw);
+              }
+              return x;
+            },
+            [&](int k, int ub, int r, bool is, float x) __attribute__((always_inline)) {
+              s.v[k][ub][r] = is ? x : s.v[k][ub][r];
+            });
       }
     } else {
       bool mine = false;
@@ -479,7 +483,7 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
   };
   // the label's element of P is negative
   auto patch = [&](uint32_t st, Probs& pb) __attribute__((always_inline)) {
-    each_hit(st, CS_LAB, [&](int k, int ub, int r, bool is, float) __attribute__((always_inline)) {
+    each_hit(st, [](int) { return f32x4{}; }, [&](int k, int ub, int r, bool is, float) __attribute__((always_inline)) {
       const uint32_t sign = is ? (r & 1 ? 0x80000000u : 0x8000u) : 0u;
 #pragma unroll
       for (int pl = 0; pl < NP; ++pl) pb.w[k >> 1][ub][pl][2 * (k & 1) + (r >> 1)] ^= sign;
