@@ -2420,4 +2420,6 @@ class DropoutFn(torch.autograd.Function):
 
 def dropout(x: torch.Tensor, rate: float, ticket: torch.Tensor) -> torch.Tensor:
     """Dropout of x with the mask of `ticket` (dropout_ticket, or an int64 [2] (seed, step) tensor)."""
+    if not 0.0 <= rate < 1.0:
+        raise ValueError(f"dropout: rate must lie in [0, 1), got {rate!r}")
     return DropoutFn.apply(x, float(rate), ticket)

@@ -476,7 +476,9 @@ class MultiTaskModel(nn.Module):
     def _compute_loss(self, data, training, return_parts, with_regularization):
         features, labels = self._split(data)
         ids = None
-        if "user_id" in features and "movie_id" in features:
+        # (towers with dropout give equal ids different rows: no grouping by id)
+        wet = getattr(self.encoder, "tower_dropout", 0.0) > 0 and self.encoder.user_tower.drops()
+        if "user_id" in features and "movie_id" in features and not wet:
             # the towers see only the ids (:85-90), so equal ids give equal embeddings: the
             # retrieval loss's deduplicated pair groups rows by id (functional.inbatch_dedup_plan)
             enc = self.encoder

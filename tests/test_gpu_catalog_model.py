@@ -147,3 +147,29 @@ def test_train_steps(cuda):
         assert not torch.equal(before[k], after[k]), k
     losses2, _, after2 = run()
     assert losses == losses2 and all(torch.equal(after[k], after2[k]) for k in after)
+
+
+def test_in_batch_loss_with_tower_dropout(cuda):
+    """The multi-task step with dropping towers: rows of one id differ, so none may share a row's result;
+    the in-batch term is the one of the towers' own outputs."""
+    models, F = pkg("models"), pkg("functional")
+    cfg = pkg("config").ModelConfig(embedding_dim=64, user_tower_dims=[32], item_tower_dims=[32], dnn_dims=[32])
+    m = models.MultiTaskModel(cfg, [str(i) for i in range(5)], [str(i) for i in range(6)], {}, device="cuda")
+    m.encoder = models.MultiTowerModel(cfg, [str(i) for i in range(5)], [str(i) for i in range(6)], {}, seed=0,
+                                       device="cuda", tower_dropout=0.5)
+    g = torch.Generator().manual_seed(2)
+    B = 300
+    feats = {"user_id": torch.randint(0, 6, (B,), generator=g).cuda(),
+             "movie_id": torch.randint(0, 7, (B,), generator=g).cuda()}
+    labels = {"rating": torch.ones(B, device="cuda"), "y_implicit": torch.ones(B, device="cuda")}
+    models.set_dropout_seed(m, 1)
+    loss, parts = m.compute_loss((feats, labels), return_parts=True)
+    loss.backward()
+    models.set_dropout_seed(m, 1)
+    out = m.encoder(feats)
+    u, c = out["user_embedding"].detach(), out["item_embedding"].detach()
+    assert not torch.equal(u[feats["user_id"] == 3][0], u[feats["user_id"] == 3][1])
+    s = u.double() @ c.double().T
+    want = float((torch.logsumexp(s, 1) - s.diagonal()).sum())
+    assert abs(float(parts["retrieval"].detach()) - want) <= 1e-5 * abs(want)
+    assert all(bool(p.grad.isfinite().all()) for p in m.encoder.user_tower.parameters())

@@ -164,6 +164,8 @@ def test_refusals(cuda):
     for rate in (-0.1, 1.0, 2.0, float("nan")):
         with pytest.raises(ValueError, match="rate"):
             F.dropout_apply(x, rate, t)
+        with pytest.raises(ValueError, match="rate"):
+            F.dropout(x, rate, t)
     with pytest.raises(pkg("_native").NativeError, match="keeps no element"):
         F.dropout_apply(x, 1 - 2.0 ** -40, t)
     with pytest.raises(TypeError):
