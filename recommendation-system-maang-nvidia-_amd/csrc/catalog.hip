@@ -137,18 +137,19 @@ enum { CS_STATS = 0, CS_ROW = 1, CS_COL = 2 };
 
 // Shape of a pass: UB 16-row subtiles of resident rows per wave, NW waves, tiles of KT streamed rows taken
 // in groups of 32 SG rows, NB tiles in LDS (the copies run NB - 1 tiles ahead), WG workgroups per CU.
-// O, the resident rows and a group's scores fill the registers, two waves a SIMD. Groups of 64 rows form
-// half as many sums and maxima as groups of 32 (8192 x 100k x 128 fp32, row pass: 0.97 against 1.19 ms); the
-// bf16 column pass has registers for a third wave at groups of 32 (16384 x 1M x 128: 6.2 against 6.8 ms).
-// At 256 columns a wave holds 16 rows; the row pass takes groups of 64 (2999 x 30011 fp32: 252 against
-// 267 us), the column pass, with its statistics, groups of 32 (290 against 318 us).
+// O, the resident rows and a group's scores fill the registers. Groups of 64 rows form half as many sums
+// and maxima as groups of 32 (8192 x 100k x 128 fp32, row pass: 0.97 against 1.19 ms). Three waves a SIMD
+// where they fit: at 64 columns (8192 x 100k, fp32 passes 0.56 and 0.58 against 0.61 and 0.68 ms), and for
+// the bf16 column pass, without a running maximum, at groups of 32 (16384 x 1M x 128: 6.2 against 6.8 ms;
+// 4096 x 60k x 256: 260 against 315 us). At 256 columns a wave holds 16 rows.
 struct CsCfg {
   int UB, NW, KT, NB, SG, WG;
 };
 constexpr CsCfg cs_cfg(int D, int NP, int MODE) {
-  if (D == 256) return MODE == CS_COL ? CsCfg{1, 8, 32, 4, 1, 1} : CsCfg{1, 8, 64, NP == 1 ? 4 : 2, 2, 1};
-  if (NP == 1 && MODE == CS_COL) return {2, 4, 64, 2, 1, 3};
-  return {2, 8, 64, NP == 2 && D == 128 ? 4 : 8, 2, 1};
+  if (D == 64) return {2, 4, 64, 3, 2, 3};
+  if (NP == 1 && MODE == CS_COL) return D == 128 ? CsCfg{2, 4, 64, 2, 1, 3} : CsCfg{1, 4, 32, 3, 1, 3};
+  if (D == 128) return {2, 8, 64, NP == 2 ? 4 : 8, 2, 1};
+  return {1, 8, 64, NP == 2 ? 2 : 4, 2, 1};
 }
 constexpr int cs_block_rows(int D, int NP, int MODE) {
   return 16 * cs_cfg(D, NP, MODE).UB * cs_cfg(D, NP, MODE).NW;
