@@ -87,6 +87,9 @@ struct CsPass {
   int64_t ld;             // its row length
   int out_bf16;
   const float* gscale;
+  const float* dx_unit;   // the forward's unit gradient of x, n_dx values: workgroups past the blocks scale it
+  int64_t n_dx;           // (one launch less than a kernel of its own)
+  void* dx;
 };
 
 template <int NP>
@@ -168,6 +171,23 @@ __device__ __forceinline__ void cs_wait() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"i"(N) : "memory");
 }
 
+// dx = c g / Z times the forward's unit gradient, `threads` values of 4 a workgroup
+__device__ __forceinline__ void cs_dx(int64_t blk, int threads, const float* __restrict__ u, int64_t n, float scale,
+                                      const CsScal* scal, const float* gscale, void* __restrict__ out, int bf16) {
+  const float f = scale * scal->inv_z * (gscale ? *gscale : 1.f);
+  const int64_t i = (blk * threads + threadIdx.x) * 4;
+  if (i + 4 <= n) {
+    const f32x4 v = *reinterpret_cast<const f32x4*>(u + i) * f;
+    if (bf16) *reinterpret_cast<u32x2*>((__bf16*)out + i) = u32x2{ib_pk(v[0], v[1]), ib_pk(v[2], v[3])};
+    else *reinterpret_cast<f32x4*>((float*)out + i) = v;
+  } else {
+    for (int64_t j = i; j < n; ++j) {
+      if (bf16) ((__bf16*)out)[j] = (__bf16)(u[j] * f);
+      else ((float*)out)[j] = u[j] * f;
+    }
+  }
+}
+
 template <int D, int NP, int MODE>
 __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) void cs_pass_kernel(CsPass p) {
   constexpr int UB = cs_cfg(D, NP, MODE).UB, NW = cs_cfg(D, NP, MODE).NW, KT = cs_cfg(D, NP, MODE).KT;
@@ -178,8 +198,13 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
   __shared__ __attribute__((aligned(1024))) char smem[NB * BUF];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4, i16 = lane & 15;
+  const int grid = p.full + p.nrb * p.nsplit;
+  if (MODE == CS_COL && (int)blockIdx.x >= grid) {
+    cs_dx(blockIdx.x - grid, 64 * NW, p.dx_unit, p.n_dx, p.scale, p.scal, p.gscale, p.dx, p.out_bf16);
+    return;
+  }
   const bool whole = (int)blockIdx.x < p.full;
-  const int id = whole ? cs_xcd(blockIdx.x, p.full) : cs_xcd(blockIdx.x - p.full, gridDim.x - p.full);
+  const int id = whole ? cs_xcd(blockIdx.x, p.full) : cs_xcd(blockIdx.x - p.full, grid - p.full);
   const int split = whole ? 0 : id / p.nrb;
   const int64_t r0 = (int64_t)(whole ? id : p.full + id % p.nrb) * cs_block_rows(D, NP, MODE) + wave * (16 * UB);
   const int64_t per = whole ? p.tiles : p.per;
@@ -632,6 +657,7 @@ struct CsFew {
   float kbase;
   int32_t* lab;
   float *m, *l;
+  unsigned int* done;
 };
 template <int DP, int Q>
 __global__ __launch_bounds__(256) void cs_few_kernel(CsFew p) {
@@ -648,6 +674,7 @@ __global__ __launch_bounds__(256) void cs_few_kernel(CsFew p) {
       if (d < p.D) v[c] = *reinterpret_cast<const f32x4*>(row + d);
     }
   };
+  if (blockIdx.x == 0) ticket_zero(p.done, threadIdx.x, 256);
   f32x4 xq[Q][NC];
   int32_t lab[Q];
   float m[Q], l[Q];
@@ -773,6 +800,7 @@ struct CsImage {
   float* kx;
   const float* part;
   CsScal* scal;
+  unsigned int* done;
   int xblocks;
 };
 
@@ -793,7 +821,10 @@ __global__ __launch_bounds__(256) void cs_image_kernel(CsImage p) {
     wscale = ldexpf(1.f, e);
     if ((int)blockIdx.x == p.xblocks && threadIdx.x == 0) p.scal->w_inv = ldexpf(1.f, -e);
   }
-  if (blockIdx.x == 0 && threadIdx.x < 4) p.scal->zero[threadIdx.x] = 0.f;
+  if (blockIdx.x == 0) {
+    if (threadIdx.x < 4) p.scal->zero[threadIdx.x] = 0.f;
+    ticket_zero(p.done, threadIdx.x, 256);
+  }
   const int64_t blk = is_x ? blockIdx.x : blockIdx.x - p.xblocks;
   const int64_t nblk = is_x ? p.xblocks : gridDim.x - p.xblocks;
   const int64_t rows = is_x ? p.N : p.V, rows_pad = is_x ? p.Npad : p.V;
@@ -876,19 +907,63 @@ struct CsRows {
   const int32_t* lab;
   const float* weights;
   const float* kx;
-  const CsScal* scal;
   float scale, kbase;
   float *row, *lse, *dx, *stat;
+  CsScal* scal;
+  unsigned int* done;  // completion tickets (ticket_last)
+  int mean;
+  float* loss;
 };
 __device__ __forceinline__ float cs_ld(const void* x, int bf16, int64_t i) {
   return bf16 ? (float)((const __bf16*)x)[i] : ((const float*)x)[i];
 }
 
+// the loss, 1 / Z and whether a weight is negative: one workgroup of at most 512 threads, fixed order. The
+// row losses may come from other workgroups of the same grid.
+__device__ __forceinline__ void cs_total(const CsRows& p) {
+  __shared__ double sh[2][8];
+  __shared__ int neg;
+  const int threads = blockDim.x, waves = threads / 64;
+  if (threadIdx.x == 0) neg = 0;
+  __syncthreads();
+  double s = 0., z = 0.;
+  bool below = false;
+#pragma unroll 8
+  for (int64_t n = threadIdx.x; n < p.N; n += threads) {
+    const bool in = p.lab[n] != -1;
+    const float a = p.weights ? p.weights[n] : 1.f;
+    const float r = __hip_atomic_load(p.row + n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    below |= in && a < 0.f;
+    s += in ? (double)a * (double)r : 0.;
+    z += in ? (double)a : 0.;
+  }
+  if (below) neg = 1;
+  s = wave_sum_d(s);
+  z = wave_sum_d(z);
+  if ((threadIdx.x & 63) == 0) {
+    sh[0][threadIdx.x >> 6] = s;
+    sh[1][threadIdx.x >> 6] = z;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    s = z = 0.;
+    for (int i = 0; i < waves; ++i) {
+      s += sh[0][i];
+      z += sh[1][i];
+    }
+    const double inv = !p.mean ? 1. : z != 0. ? 1. / z : 0.;
+    p.scal->inv_z = (float)inv;
+    p.scal->neg = neg;
+    *p.loss = (float)(s * inv);
+  }
+}
+__global__ __launch_bounds__(64) void cs_no_rows_kernel(CsRows p) { cs_total(p); }
+
 // Joins the splits of a row: NWV waves per row (1: four rows per workgroup), DP / 4 lanes per split, the
 // splits dealt to the lane groups and their sums joined in a fixed order. Then the label's logit (64-bit
 // sums), the row's loss, its statistics for the column pass and its unit gradient a q (O / l - w_y).
 template <int DP, int NP, int NWV>
-__global__ __launch_bounds__(NWV == 1 ? 256 : 64 * NWV) void cs_rows_kernel(CsRows p) {
+__device__ __forceinline__ void cs_row(const CsRows& p) {
   constexpr int LPR = DP / 4, GW = 64 / LPR, G = NWV * GW;
   __shared__ f32x4 sh[NWV][LPR];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -961,7 +1036,8 @@ __global__ __launch_bounds__(NWV == 1 ? 256 : 64 * NWV) void cs_rows_kernel(CsRo
   const float q = t > 0.f ? 1.f / (1.f + et) : et / (1.f + et);  // NaN stays NaN
   const double lse2 = lb >= 0 ? fmax(o2, sy) + (double)soft * CS_LOG2E : o2;
   if (lane == 0) {
-    p.row[n] = lb >= 0 ? soft + fmaxf(t, 0.f) : lb == -1 ? 0.f : NAN;
+    __hip_atomic_store(p.row + n, lb >= 0 ? soft + fmaxf(t, 0.f) : lb == -1 ? 0.f : NAN, __ATOMIC_RELAXED,
+                       __HIP_MEMORY_SCOPE_AGENT);  // the grid's last workgroup sums them
     p.lse[n] = (float)(lse2 * CS_LN2);
   }
   if (lane == 0 && p.stat) {  // a column pass follows
@@ -986,62 +1062,20 @@ __global__ __launch_bounds__(NWV == 1 ? 256 : 64 * NWV) void cs_rows_kernel(CsRo
   }
 }
 
-// the loss, 1 / Z and whether a weight is negative; one workgroup, fixed order
-__global__ __launch_bounds__(1024) void cs_total_kernel(const float* __restrict__ row, const int32_t* __restrict__ lab,
-                                                         const float* __restrict__ weights, int64_t N, int mean,
-                                                         CsScal* scal, float* __restrict__ loss) {
-  __shared__ double sh[2][16];
-  __shared__ int neg;
-  if (threadIdx.x == 0) neg = 0;
+// The rows, and in the grid's last workgroup the total: 4 to 6 us more than the rows alone where a kernel of
+// its own took 4 and a launch (20 and 11 at 16384 rows of 14 ms).
+template <int DP, int NP, int NWV>
+__global__ __launch_bounds__(NWV == 1 ? 256 : 64 * NWV) void cs_rows_kernel(CsRows p) {
+  cs_row<DP, NP, NWV>(p);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's row losses are out
   __syncthreads();
-  double s = 0., z = 0.;
-  bool below = false;
-#pragma unroll 4
-  for (int64_t n = threadIdx.x; n < N; n += 1024) {
-    const bool in = lab[n] != -1;
-    const float a = weights ? weights[n] : 1.f, r = row[n];
-    below |= in && a < 0.f;
-    s += in ? (double)a * (double)r : 0.;
-    z += in ? (double)a : 0.;
-  }
-  if (below) neg = 1;
-  s = wave_sum_d(s);
-  z = wave_sum_d(z);
-  if ((threadIdx.x & 63) == 0) {
-    sh[0][threadIdx.x >> 6] = s;
-    sh[1][threadIdx.x >> 6] = z;
-  }
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    s = z = 0.;
-    for (int i = 0; i < 16; ++i) {
-      s += sh[0][i];
-      z += sh[1][i];
-    }
-    const double inv = !mean ? 1. : z != 0. ? 1. / z : 0.;
-    scal->inv_z = (float)inv;
-    scal->neg = neg;
-    *loss = (float)(s * inv);
-  }
+  if (ticket_last(p.done, blockIdx.x, gridDim.x)) cs_total(p);
 }
 
 // ---- backward ------------------------------------------------------------------------------------
-// dx = c g / Z times the forward's unit gradient
-__global__ __launch_bounds__(256) void cs_dx_kernel(const float* __restrict__ u, int64_t n, float scale,
-                                                    const CsScal* __restrict__ scal, const float* __restrict__ gscale,
-                                                    void* __restrict__ out, int bf16) {
-  const float f = scale * scal->inv_z * (gscale ? *gscale : 1.f);
-  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
-  if (i + 4 <= n) {
-    const f32x4 v = *reinterpret_cast<const f32x4*>(u + i) * f;
-    if (bf16) *reinterpret_cast<u32x2*>((__bf16*)out + i) = u32x2{ib_pk(v[0], v[1]), ib_pk(v[2], v[3])};
-    else *reinterpret_cast<f32x4*>((float*)out + i) = v;
-  } else {
-    for (int64_t j = i; j < n; ++j) {
-      if (bf16) ((__bf16*)out)[j] = (__bf16)(u[j] * f);
-      else ((float*)out)[j] = u[j] * f;
-    }
-  }
+__global__ __launch_bounds__(256) void cs_dx_kernel(const float* u, int64_t n, float scale, const CsScal* scal,
+                                                    const float* gscale, void* out, int bf16) {
+  cs_dx(blockIdx.x, 256, u, n, scale, scal, gscale, out, bf16);
 }
 
 // dw from the column pass's partials of several row ranges, in their order
@@ -1176,11 +1210,13 @@ struct CsKeep {
   }
 };
 struct CsFwdWs {
+  unsigned int* done;
   float *part, *m, *l, *O;
   bool ok;
   size_t bytes;
   CsFwdWs(void* base, size_t size, const CsShape& s, int want) {
     Carve c(base, size);
+    done = c.take<unsigned int>(TICKET_WORDS);
     part = c.take<float>(CS_AMAX_BLOCKS);
     m = c.take<float>((size_t)s.rsplit * s.N);
     l = c.take<float>((size_t)s.rsplit * s.N);
@@ -1263,7 +1299,7 @@ extern "C" int rs_catalog_softmax_fwd(const void* X, const void* W, const int64_
   hipStream_t st = as_stream(stream);
   const float kbase = (float)((double)scale * CS_LOG2E);
   if (N > 0 && s.few) {
-    const CsFew f{(const float*)X, (const float*)W, labels, N, V, D, ignore_index, s.rtiles, kbase, k.lab, w.m, w.l};
+    const CsFew f{(const float*)X, (const float*)W, labels, N, V, D, ignore_index, s.rtiles, kbase, k.lab, w.m, w.l, w.done};
     const int Q = (int)ceil_div(N, 16);
 #define CS_GO(WD, QQ)                                          \
   if (s.DP == WD && (Q == QQ || (QQ == 4 && Q == 3)))          \
@@ -1275,7 +1311,7 @@ extern "C" int rs_catalog_softmax_fwd(const void* X, const void* W, const int64_
     if (s.NP == 2) hipLaunchKernelGGL(cs_amax_kernel, dim3(CS_AMAX_BLOCKS), dim3(256), 0, st, (const float*)W, V * D, w.part);
     const int rpb = 256 / (s.DP / 4);
     CsImage im{X,    W,    k.ximg, k.wimg, N, s.Npad, V, D, s.Npad * s.DP * 2, V * s.DP * 2, ignore_index, labels, k.lab,
-               k.kx, w.part, k.scal, 0};
+               k.kx, w.part, k.scal, w.done, 0};
     int64_t xb = ceil_div(s.Npad, rpb), wb = s.wimage ? ceil_div(V, rpb) : 0;
     im.xblocks = (int)(xb < 2048 ? xb : 2048);
     if (wb > 4096) wb = 4096;
@@ -1313,9 +1349,9 @@ extern "C" int rs_catalog_softmax_fwd(const void* X, const void* W, const int64_
     if (want & RS_CATALOG_DX) cs_launch_pass<CS_ROW>(s, p, s.rnrb * s.rsplit, st);
     else cs_launch_pass<CS_STATS>(s, p, s.rnrb * s.rsplit, st);
   }
+  const CsRows r{X, W, s.NP == 1, N, s.Npad, V, D, s.rsplit, w.m, w.l, w.O, k.lab, weights, k.kx, scale, kbase, row_loss,
+                 lse, k.dx, want & RS_CATALOG_DW ? k.stat : nullptr, k.scal, w.done, mean, loss};
   if (N > 0) {
-    CsRows r{X, W, s.NP == 1, N, s.Npad, V, D, s.rsplit, w.m, w.l, w.O, k.lab, weights, k.kx, k.scal, scale, kbase,
-             row_loss, lse, k.dx, want & RS_CATALOG_DW ? k.stat : nullptr};
     // many splits of few rows: a workgroup per row, else a wave
     const int wide = s.rsplit > 64 ? 8 : s.rsplit > 8 ? 4 : 0;
     const dim3 gr((unsigned)(wide ? s.Npad : s.Npad / 4));
@@ -1328,7 +1364,7 @@ extern "C" int rs_catalog_softmax_fwd(const void* X, const void* W, const int64_
     CS_GO(64, 1) CS_GO(64, 2) CS_GO(128, 1) CS_GO(128, 2) CS_GO(256, 1) CS_GO(256, 2)
 #undef CS_GO
   }
-  hipLaunchKernelGGL(cs_total_kernel, dim3(1), dim3(1024), 0, st, row_loss, k.lab, weights, N, mean, k.scal, loss);
+  if (N == 0) hipLaunchKernelGGL(cs_no_rows_kernel, dim3(1), dim3(64), 0, st, r);
   return check_launch("catalog_softmax_fwd");
 }
 
@@ -1350,7 +1386,7 @@ extern "C" int rs_catalog_softmax_bwd(const void* W, int64_t N, int64_t V, int64
     return RS_ERR_WORKSPACE;
   }
   hipStream_t st = as_stream(stream);
-  if (dX && N > 0)
+  if (dX && N > 0 && !dW)
     hipLaunchKernelGGL(cs_dx_kernel, dim3((unsigned)ceil_div(N * D, 1024)), dim3(256), 0, st, k.dx, N * D, scale, k.scal,
                        gscale, dX, s.NP == 1);
   if (dW) {
@@ -1383,7 +1419,14 @@ extern "C" int rs_catalog_softmax_bwd(const void* W, int64_t N, int64_t V, int64
     p.ld = D;
     p.out_bf16 = s.NP == 1;
     p.gscale = gscale;
-    cs_launch_pass<CS_COL>(s, p, p.full + (int64_t)p.nrb * p.nsplit, st);
+    int64_t grid = p.full + (int64_t)p.nrb * p.nsplit;
+    if (dX && N > 0) {
+      p.dx_unit = k.dx;
+      p.n_dx = N * D;
+      p.dx = dX;
+      grid += ceil_div(N * D, 256 * cs_cfg(s.DP, s.NP, CS_COL).NW);
+    }
+    cs_launch_pass<CS_COL>(s, p, grid, st);
     if (s.prows > 0) {
       void* out = (char*)dW + (V - s.prows) * D * s.es;
       const dim3 gd((unsigned)ceil_div(s.prows, 256 / (s.DP / 4)));
