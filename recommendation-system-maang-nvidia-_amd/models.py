@@ -106,7 +106,9 @@ class Embedding(nn.Module):
 class Dropout(nn.Module):
     """keras.layers.Dropout(rate): in training, elements are dropped by a counter-based generator (seed,
     step) kept on the device and advanced once per call, so a step captured in a graph draws a new mask
-    at each replay; no mask is stored (functional.dropout). Outside training the identity."""
+    at each replay; no mask is stored (functional.dropout). Outside training the identity.
+    A forward that is run again (activation checkpointing) draws the next mask: such code takes one
+    ticket for both runs and calls functional.dropout."""
 
     def __init__(self, rate: float, seed: int = 0, device=None):
         super().__init__()
@@ -394,15 +396,17 @@ class MultiTowerModel(nn.Module):
 # MultiTaskModel (src/models.py:105-159)
 # --------------------------------------------------------------------------------------------
 class MultiTaskModel(nn.Module):
-    """Two towers -> in-batch retrieval loss and [u || i] -> DCN -> rating / CTR heads."""
+    """Two towers -> in-batch retrieval loss and [u || i] -> DCN -> rating / CTR heads. tower_dropout:
+    MultiTowerModel's, drawn by compute_loss(training=True)."""
 
     def __init__(self, config: ModelConfig, user_vocab: List[str], item_vocab: List[str],
                  feature_specs: Dict[str, Any], class_weights: Dict[int, float] = None,
-                 seed: int = 0, device=None):
+                 seed: int = 0, device=None, tower_dropout: float = 0.0):
         super().__init__()
         device = device or _default_device()
         self.config = config
-        self.encoder = MultiTowerModel(config, user_vocab, item_vocab, feature_specs, seed=seed, device=device)
+        self.encoder = MultiTowerModel(config, user_vocab, item_vocab, feature_specs, seed=seed, device=device,
+                                       tower_dropout=tower_dropout)
         self.class_weights = dict(class_weights) if class_weights else None
         d = 2 * config.embedding_dim
         self.dcn = DeepCrossNetwork(config.cross_layers, config.dnn_dims, config.dropout_rate, config.l2_reg,
@@ -425,15 +429,15 @@ class MultiTaskModel(nn.Module):
             return v.to(self.encoder.device, dtype=torch.float32, non_blocking=True).reshape(-1).contiguous()
         return torch.as_tensor(np.asarray(v, dtype=np.float32), device=self.encoder.device).reshape(-1)
 
-    def _towers(self, features, orders=None):
-        emb = self.encoder(features, orders=orders)
+    def _towers(self, features, orders=None, training=None):
+        emb = self.encoder(features, training, orders)
         return emb["user_embedding"], emb["item_embedding"]
 
     # ---- keras call / compute_loss -----------------------------------------------------------
     def forward(self, data, training=None):
         """MultiTaskModel.call (src/models.py:125-131)."""
         features, _ = self._split(data)
-        u, i = self._towers(features)
+        u, i = self._towers(features, training=training)
         _, xl, h = self.dcn.forward_pair(u, i)
         r, p = HeadsFn.apply(xl, h, self.rating_head.kernel, self.rating_head.bias,
                              self.ctr_head.kernel, self.ctr_head.bias)
@@ -477,7 +481,7 @@ class MultiTaskModel(nn.Module):
         features, labels = self._split(data)
         ids = None
         # (towers with dropout give equal ids different rows: no grouping by id)
-        wet = getattr(self.encoder, "tower_dropout", 0.0) > 0 and self.encoder.user_tower.drops()
+        wet = getattr(self.encoder, "tower_dropout", 0.0) > 0 and training
         if "user_id" in features and "movie_id" in features and not wet:
             # the towers see only the ids (:85-90), so equal ids give equal embeddings: the
             # retrieval loss's deduplicated pair groups rows by id (functional.inbatch_dedup_plan)
@@ -522,7 +526,7 @@ class MultiTaskModel(nn.Module):
                 self.config.contraction_precision, ids[4], uid, iid, enc.user_embedding.weight,
                 enc.item_embedding.weight, *params)
         else:
-            u, i = self._towers(features, orders)
+            u, i = self._towers(features, orders, training)
         # the retrieval task (:137) and the concat + cross stack (:128, 38-44) read the same tower
         # outputs: one node, whose backward adds the retrieval gradient inside the cross kernel
         ret, _, x0, xl = RetrievalCrossFn.apply(u, i, self.dcn.cross_w, self.dcn.cross_b,

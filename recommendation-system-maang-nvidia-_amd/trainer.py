@@ -114,6 +114,11 @@ def balanced_class_weights(y) -> Dict[int, float]:
     return out
 
 
+def _embed(encoder, features):
+    """The encoder's embeddings outside training: without its towers' dropout, where it has one."""
+    return encoder(features, training=False) if getattr(encoder, "tower_dropout", 0.0) > 0 else encoder(features)
+
+
 class EarlyStopping:
     """keras.callbacks.EarlyStopping(monitor, patience, restore_best_weights=True) (src/trainer.py:166)
     together with ModelCheckpoint(save_best_only=True) (:167): ``on_epoch_end`` returns
@@ -325,7 +330,7 @@ class ProductionTrainer:
         (r0, r1) limits it to vocab rows [r0, r1) (a shard)."""
         r0, r1 = rows if rows is not None else (0, len(item_vocab))
         ids = torch.arange(r0 + 1, r1 + 1, dtype=torch.int64, device=self.device)
-        out = [model.encoder({"movie_id": ids[i:i + 512]})["item_embedding"] for i in range(0, len(ids), 512)]
+        out = [_embed(model.encoder, {"movie_id": ids[i:i + 512]})["item_embedding"] for i in range(0, len(ids), 512)]
         if not out:
             return torch.empty((0, self.config.embedding_dim), dtype=torch.float32, device=self.device)
         return torch.cat(out).contiguous()
@@ -350,7 +355,7 @@ class ProductionTrainer:
         else:
             index = self._get_item_embeddings(model, item_vocab)
         sample = val_df.sample(n=min(1000, len(val_df)), random_state=42)
-        user_embs = model.encoder({"user_id": sample["user_id"].values})["user_embedding"].contiguous()
+        user_embs = _embed(model.encoder, {"user_id": sample["user_id"].values})["user_embedding"].contiguous()
         true_rows = model.encoder.item_lookup(sample["movie_id"].values) - 1   # -1: not in vocab
         metrics = recall_at_k(index, user_embs, true_rows, self.config.eval_topk)
         logger.info(f"Evaluation Results: {metrics}")

@@ -154,16 +154,15 @@ def test_in_batch_loss_with_tower_dropout(cuda):
     the in-batch term is the one of the towers' own outputs."""
     models, F = pkg("models"), pkg("functional")
     cfg = pkg("config").ModelConfig(embedding_dim=64, user_tower_dims=[32], item_tower_dims=[32], dnn_dims=[32])
-    m = models.MultiTaskModel(cfg, [str(i) for i in range(5)], [str(i) for i in range(6)], {}, device="cuda")
-    m.encoder = models.MultiTowerModel(cfg, [str(i) for i in range(5)], [str(i) for i in range(6)], {}, seed=0,
-                                       device="cuda", tower_dropout=0.5)
+    m = models.MultiTaskModel(cfg, [str(i) for i in range(5)], [str(i) for i in range(6)], {}, device="cuda",
+                              tower_dropout=0.5)
     g = torch.Generator().manual_seed(2)
     B = 300
     feats = {"user_id": torch.randint(0, 6, (B,), generator=g).cuda(),
              "movie_id": torch.randint(0, 7, (B,), generator=g).cuda()}
     labels = {"rating": torch.ones(B, device="cuda"), "y_implicit": torch.ones(B, device="cuda")}
     models.set_dropout_seed(m, 1)
-    loss, parts = m.compute_loss((feats, labels), return_parts=True)
+    loss, parts = m.compute_loss((feats, labels), training=True, return_parts=True)
     loss.backward()
     models.set_dropout_seed(m, 1)
     out = m.encoder(feats)
@@ -173,3 +172,16 @@ def test_in_batch_loss_with_tower_dropout(cuda):
     want = float((torch.logsumexp(s, 1) - s.diagonal()).sum())
     assert abs(float(parts["retrieval"].detach()) - want) <= 1e-5 * abs(want)
     assert all(bool(p.grad.isfinite().all()) for p in m.encoder.user_tower.parameters())
+    # outside training (a validation step, the exported embeddings) no row is dropped, whatever the module's mode
+    states = [d.state.clone() for d in m.modules() if isinstance(d, models.Dropout)]
+    plain = models.MultiTaskModel(cfg, [str(i) for i in range(5)], [str(i) for i in range(6)], {}, device="cuda")
+    plain.load_state_dict({k: v for k, v in m.state_dict().items() if "dropouts" not in k})
+    with torch.no_grad():
+        want = plain.compute_loss((feats, labels), training=False)
+        assert torch.equal(m.compute_loss((feats, labels), training=False), want)
+        want = plain.encoder(feats)
+        got = pkg("trainer")._embed(m.encoder, feats)
+        pred = m((feats, labels), training=False)["user_embedding"]
+    assert torch.equal(got["item_embedding"], want["item_embedding"]) and torch.equal(pred, want["user_embedding"])
+    assert all(torch.equal(a, d.state) for a, d in
+               zip(states, (d for d in m.modules() if isinstance(d, models.Dropout))))
