@@ -807,10 +807,12 @@ int rs_l2_normalize_rows_f32(const float* x, int64_t n, int64_t D, float* out, r
 
 /* ---- softmax cross entropy over a whole catalogue ---------------------------------------------
  * The full-catalogue form of the retrieval loss (tfrs.tasks.Retrieval, src/models.py:116,137, whose
- * vocabulary is the batch's own items). X [N][D] rows, W [V][D] items (D <= 256; both RS_DTYPE_F32 or
- * both RS_DTYPE_BF16), labels [N] in [0, V) or ignore_index, scale c in [2^-60, 2^60], weights a [N] (nullable: 1):
+ * vocabulary is the batch's own items). X [N][D] rows, W [V][D] items (D <= 256, N < 2^26, V < 2^29; both
+ * RS_DTYPE_F32 or both RS_DTYPE_BF16), labels [N] in [0, V) or ignore_index, scale c in [2^-60, 2^60],
+ * weights a [N] (nullable: 1):
  *   s_nv = c <x_n, w_v>, lse_n = log sum_v exp s_nv, row_n = lse_n - s_n,label, loss = sum a_n row_n / Z,
- * Z = 1, or with `mean` the sum of a over the labelled rows (no labelled row: loss 0). No logits are
+ * Z = 1, or with `mean` the sum of a over the labelled rows (a sum of zero, or no labelled row: loss 0).
+ * No logits are
  * stored. An ignored row has row_loss 0, enters neither loss nor gradients (whatever its x holds) and
  * has the lse of its finite entries; a label that is neither in range nor ignore_index makes its row
  * loss, its dX row and the loss NaN and stays out of dW. row_loss, lse [N] and *loss are fp32.
@@ -836,7 +838,7 @@ int rs_catalog_softmax_bwd(const void* W, int64_t N, int64_t V, int64_t D, int d
  * keras.layers.Dropout (the reference's dropout_rate, src/config.py:21, src/models.py:16,22): y = x /
  * (1 - rate) where element i's word is at least round(rate 2^32), else 0. Words: Philox4x32-10 with key =
  * ticket[0] and counter (i / 4, ticket[1]), word i % 4; ticket is int64 [2] on the device. The backward is
- * the same call on dy with the same ticket. x and y hold n elements of dtype; y may be x.
+ * the same call on dy with the same ticket. x and y hold n < 2^35 elements of dtype; y may be x.
  * rs_dropout_ticket copies state (int64 [2]: seed, step) to ticket and adds one to the step, on the
  * device, so a captured step draws a new mask at each replay. */
 int rs_dropout(const void* x, int64_t n, int dtype, double rate, const int64_t* ticket, void* y, rs_stream_t stream);

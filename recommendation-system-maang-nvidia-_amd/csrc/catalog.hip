@@ -1129,8 +1129,10 @@ CsSpread cs_spread(int64_t nrb, int64_t tiles, const CsCfg& c, int D, int NP, in
   if (nrb < 1 || tiles < 1) return best;
   double best_cost = 1e300;
   // the column pass writes a whole block's gradient itself: whole rounds of blocks need no partials
-  for (int64_t full : {(int64_t)0, col ? nrb / slots * slots : (int64_t)0, col ? nrb : (int64_t)0}) {
-    const int64_t rest = nrb - full;
+  const int64_t fulls[3] = {0, nrb / slots * slots, nrb};
+  for (int i = 0; i < (col ? 3 : 1); ++i) {
+    const int64_t full = fulls[i], rest = nrb - full;
+    if (i > 0 && full == fulls[i - 1]) continue;
     const double base = (double)ceil_div(full, slots) * (tiles * tile + 6.);
     const int64_t part = rows - full * block;
     // over the distinct splits, coarsest first
@@ -1157,7 +1159,7 @@ struct CsShape {
   int64_t rtiles, rper, ctiles, rnrb, cnrb;
   int64_t prows;  // the column pass's rows with partials
 };
-CsShape cs_shape(int64_t N, int64_t V, int64_t D, int dtype, int want) {
+CsShape cs_plan(int64_t N, int64_t V, int64_t D, int dtype, int want) {
   CsShape s;
   s.N = N;
   s.V = V;
@@ -1187,6 +1189,19 @@ CsShape cs_shape(int64_t N, int64_t V, int64_t D, int dtype, int want) {
   }
   s.rper = ceil_div(s.rtiles, s.rsplit);
   return s;
+}
+// the plan of the sizes, kept from one call for the next of equal sizes (a forward and its backward; the
+// search takes 1 to 4 us of the host's time)
+const CsShape& cs_shape(int64_t N, int64_t V, int64_t D, int dtype, int want) {
+  struct Last {
+    int64_t N, V, D;
+    int dtype, want;
+    CsShape s;
+  };
+  static thread_local Last last{-1, 0, 0, 0, 0, {}};
+  if (last.N != N || last.V != V || last.D != D || last.dtype != dtype || last.want != want)
+    last = Last{N, V, D, dtype, want, cs_plan(N, V, D, dtype, want)};
+  return last.s;
 }
 
 struct CsKeep {
@@ -1251,7 +1266,10 @@ void cs_launch_pass(const CsShape& s, const CsPass& p, int64_t grid, hipStream_t
 int cs_check(int64_t N, int64_t V, int64_t D, int dtype, float scale, int want, const char* what) {
   RS_REQUIRE(N >= 0 && V >= 1 && D >= 1, "%s: bad sizes N=%lld V=%lld D=%lld", what, (long long)N, (long long)V,
              (long long)D);
-  RS_REQUIRE(N < (1ll << 30) && V < (1ll << 30), "%s: N and V must be below 2^30", what);
+  // labels in 31 bits; grids below 2^32 threads: the row join's 64 a row, the column pass's 4 an item at most,
+  // with one for 4 values of x
+  RS_REQUIRE(N < (1ll << 26) && V < (1ll << 29), "%s: N must be below 2^26, V below 2^29", what);
+  RS_REQUIRE(N * D < (1ll << 33), "%s: X must hold fewer than 2^33 values", what);
   RS_REQUIRE(dtype == RS_DTYPE_F32 || dtype == RS_DTYPE_BF16, "%s: unknown dtype %d", what, dtype);
   RS_REQUIRE(scale >= 0x1p-60f && scale <= 0x1p60f, "%s: scale must lie between 2^-60 and 2^60", what);
   RS_REQUIRE((want & ~(RS_CATALOG_DX | RS_CATALOG_DW)) == 0, "%s: unknown gradient flags %d", what, want);
@@ -1274,7 +1292,7 @@ extern "C" size_t rs_catalog_softmax_keep_bytes(int64_t N, int64_t V, int64_t D,
 
 extern "C" size_t rs_catalog_softmax_workspace_bytes(int64_t N, int64_t V, int64_t D, int dtype, int want) {
   if (cs_check(N, V, D, dtype, 1.f, want, "catalog_softmax") != RS_OK) return 0;
-  const CsShape s = cs_shape(N, V, D, dtype, want);
+  const CsShape& s = cs_shape(N, V, D, dtype, want);
   const size_t a = CsFwdWs(nullptr, 0, s, want).bytes, b = CsBwdWs(nullptr, 0, s, want).bytes;
   return a > b ? a : b;
 }
@@ -1289,7 +1307,7 @@ extern "C" int rs_catalog_softmax_fwd(const void* X, const void* W, const int64_
              "catalog_softmax_fwd: null pointer");
   RS_REQUIRE(aligned16(X) && aligned16(W) && aligned16(keep) && aligned16(workspace),
              "catalog_softmax_fwd: X, W, keep and workspace must be 16-byte aligned");
-  const CsShape s = cs_shape(N, V, D, dtype, want);
+  const CsShape& s = cs_shape(N, V, D, dtype, want);
   const CsKeep k(keep, keep_bytes, s, want);
   const CsFwdWs w(workspace, workspace_bytes, s, want);
   if (!k.ok || !w.ok) {
@@ -1378,7 +1396,7 @@ extern "C" int rs_catalog_softmax_bwd(const void* W, int64_t N, int64_t V, int64
   RS_REQUIRE(!dW || (want & RS_CATALOG_DW), "catalog_softmax_bwd: dW needs a forward with RS_CATALOG_DW");
   RS_REQUIRE(aligned16(W) && aligned16(keep) && aligned16(workspace) && aligned16(dX) && aligned16(dW),
              "catalog_softmax_bwd: W, keep, workspace, dX and dW must be 16-byte aligned");
-  const CsShape s = cs_shape(N, V, D, dtype, want);
+  const CsShape& s = cs_shape(N, V, D, dtype, want);
   const CsKeep k(const_cast<void*>(keep), keep_bytes, s, want);
   const CsBwdWs w(workspace, workspace_bytes, s, want);
   if (!k.ok || !w.ok) {

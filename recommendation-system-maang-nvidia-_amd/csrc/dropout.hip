@@ -105,7 +105,7 @@ extern "C" int rs_dropout(const void* x, int64_t n, int dtype, double rate, cons
   RS_REQUIRE(thr < 4294967296., "dropout: rate %.12g keeps no element of 2^32", rate);
   if (n == 0) return RS_OK;
   RS_REQUIRE(x && y && ticket, "dropout: null pointer");
-  RS_REQUIRE(n <= (1ll << 31) * 256 * 8 - 2048, "dropout: %lld elements are too many", (long long)n);
+  RS_REQUIRE(n < (1ll << 35) - 2048, "dropout: %lld elements are 2^35 or more", (long long)n);  // 2^32 threads
   const dim3 grid((unsigned)ceil_div(n, 2048));
   const float f = (float)(1. / (1. - rate));
   const bool vec = aligned16(x) && aligned16(y);

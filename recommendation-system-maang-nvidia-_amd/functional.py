@@ -2376,10 +2376,11 @@ class CatalogSoftmaxFn(torch.autograd.Function):
     def forward(ctx, X, W, labels, weights, scale: float, ignore_index: int, reduction: str):
         ctx.set_materialize_grads(False)
         W = W.contiguous()
-        loss, row, _, ctx.state = catalog_softmax_fwd(
+        loss, row, _, st = catalog_softmax_fwd(
             X.contiguous(), W, labels.contiguous(), scale, weights.contiguous() if weights is not None else None,
             ignore_index, reduction, want_grad=(ctx.needs_input_grad[0], ctx.needs_input_grad[1]))
-        ctx.save_for_backward(W)
+        ctx.save_for_backward(W, st.keep)   # (the state's buffer goes with the saved tensors)
+        ctx.sizes = st.N, st.V, st.D, st.dtype, st.scale, st.want
         ctx.mark_non_differentiable(row)
         return loss, row
 
@@ -2388,15 +2389,20 @@ class CatalogSoftmaxFn(torch.autograd.Function):
     def backward(ctx, g, _g_row):
         if g is None:
             return (None,) * 7
-        W, = ctx.saved_tensors
-        dX, dW = _catalog_bwd(_aligned(W), ctx.state, g.contiguous(), ctx.needs_input_grad[0], ctx.needs_input_grad[1])
+        W, keep = ctx.saved_tensors
+        dX, dW = _catalog_bwd(_aligned(W), CatalogSoftmaxState(keep, *ctx.sizes), g.contiguous(),
+                              ctx.needs_input_grad[0], ctx.needs_input_grad[1])
         return dX, dW, None, None, None, None, None
 
 
 def catalog_softmax_loss(X, W, labels, scale: float = 1.0, weights=None, ignore_index: int = -100,
                          reduction: str = "sum"):
     """(loss, row_loss) of catalog_softmax_fwd, differentiable by X and W through the loss (not by the
-    weights)."""
+    weights). With gradients disabled the loss alone is formed (want_grad=False)."""
+    if not torch.is_grad_enabled():   # (a node is not told: its needs_input_grad are the inputs' requires_grad)
+        return catalog_softmax_fwd(X.contiguous(), W.contiguous(), labels.contiguous(), scale,
+                                   weights.contiguous() if weights is not None else None, ignore_index, reduction,
+                                   want_grad=False)[:2]
     if weights is not None and weights.requires_grad:
         raise ValueError("catalog_softmax_loss: the loss is not differentiable by its weights; detach them")
     return CatalogSoftmaxFn.apply(X, W, labels, weights, scale, ignore_index, reduction)

@@ -27,9 +27,9 @@ def test_cpu_tensors_are_refused():
 
 
 @pytest.mark.parametrize("bad,match", [
-    (dict(N=-1), "bad sizes"), (dict(V=0), "bad sizes"), (dict(D=0), "bad sizes"), (dict(N=1 << 30), "2\\^30"),
-    (dict(V=1 << 30), "2\\^30"), (dict(D=257), "above 256"), (dict(dtype=7), "dtype"), (dict(scale=0.0), "scale"),
-    (dict(scale=float("nan")), "scale"), (dict(want=4), "flags"), (dict(x=None), "null"), (dict(w=None), "null"),
+    (dict(N=-1), "bad sizes"), (dict(V=0), "bad sizes"), (dict(D=0), "bad sizes"), (dict(N=1 << 26), "2\\^26"),
+    (dict(V=1 << 29), "2\\^29"), (dict(N=1 << 25, D=256), "2\\^33"), (dict(D=257), "above 256"),
+    (dict(dtype=7), "dtype"), (dict(scale=0.0), "scale"), (dict(scale=float("nan")), "scale"), (dict(want=4), "flags"), (dict(x=None), "null"), (dict(w=None), "null"),
     (dict(labels=None), "null"), (dict(x=A + 4), "aligned"), (dict(w=A + 8), "aligned"), (dict(keep=64), "keep"),
     (dict(ws=64), "workspace")])
 def test_forward_refusals(bad, match):
@@ -52,7 +52,8 @@ def test_backward_refusals():
 def test_dropout_refusals():
     N = pkg("_native")
     for args, match in (((A, -1, 0, 0.5, A, A), "bad size"), ((A, 8, 9, 0.5, A, A), "dtype"),
-                        ((A, 8, 0, 1.0, A, A), "rate"), ((A, 8, 0, -0.5, A, A), "rate"),
+                        ((A, 1 << 35, 1, 0.5, A, A), "2.35"), ((A, 8, 0, 1.0, A, A), "rate"),
+                        ((A, 8, 0, -0.5, A, A), "rate"),
                         ((A, 8, 0, float("nan"), A, A), "rate"), ((A, 8, 0, 1 - 2.0 ** -40, A, A), "keeps no element"),
                         ((None, 8, 0, 0.5, A, A), "null")):
         with pytest.raises(N.NativeError, match=match):
@@ -71,6 +72,36 @@ def test_workspace_queries():
             assert both >= none + 4 * n * d
             assert q("rs_catalog_softmax_workspace_bytes", n, v, d, dt, 3) > 0
     assert q("rs_catalog_softmax_keep_bytes", 4, 4, 300, 0, 0) == 0   # unsupported width
+    # sizes whose grids would pass 2^32 threads
+    for n, v, d in ((1 << 26, 4, 1), (4, 1 << 29, 1), (1 << 25, 4, 256)):
+        assert q("rs_catalog_softmax_keep_bytes", n, v, d, 1, 0) == 0
+        assert q("rs_catalog_softmax_keep_bytes", n - 1 if n > v else n, v - 1 if v > n else v, d, 1, 0) > 0
+    # the same sizes, other types and gradients: each its own plan
+    ask = [(dt, w) for dt in (0, 1) for w in (0, 1, 2, 3)]
+    first = [q("rs_catalog_softmax_workspace_bytes", 64, 50_000, 128, dt, w) for dt, w in ask]
+    for (dt, w), b in zip(reversed(ask), reversed(first)):
+        assert q("rs_catalog_softmax_workspace_bytes", 64, 50_000, 128, dt, w) == b
+
+
+def test_the_loss_alone_without_gradients(monkeypatch):
+    """With gradients disabled no gradient's work is asked for, though the operands require them."""
+    F = pkg("functional")
+    asked = []
+
+    def fwd(X, W, labels, scale=1.0, weights=None, ignore_index=-100, reduction="sum", want_grad=True):
+        asked.append(want_grad)
+        z = torch.zeros(())
+        keep = torch.empty(1)
+        return z, torch.zeros(X.shape[0]), None, F.CatalogSoftmaxState(keep, *X.shape, W.shape[0], X.dtype, scale, 0)
+
+    monkeypatch.setattr(F, "catalog_softmax_fwd", fwd)
+    x, w = torch.zeros((3, 8)), torch.zeros((5, 8), requires_grad=True)
+    y = torch.zeros(3, dtype=torch.int64)
+    loss, _ = F.catalog_softmax_loss(x, w, y)
+    assert loss.requires_grad and asked == [(False, True)]
+    with torch.no_grad():
+        loss, _ = F.catalog_softmax_loss(x, w, y, weights=torch.ones(3, requires_grad=True))
+    assert not loss.requires_grad and asked[1] is False
 
 
 def test_modules():
