@@ -815,7 +815,7 @@ int rs_l2_normalize_rows_f32(const float* x, int64_t n, int64_t D, float* out, r
  * No logits are
  * stored. An ignored row has row_loss 0, enters neither loss nor gradients (whatever its x holds) and
  * has the lse of its finite entries; a label that is neither in range nor ignore_index makes its row
- * loss, its dX row and the loss NaN and stays out of dW. row_loss, lse [N] and *loss are fp32.
+ * loss, its dX row and the loss NaN and stays out of dW. row_loss, lse [N] (nullable) and *loss are fp32.
  * want: RS_CATALOG_DX / _DW: which gradients a backward will be asked for (0: the loss alone, about
  * half the work). `keep` (rs_catalog_softmax_keep_bytes, same arguments) carries the forward's state to
  * the backward and is only read there; the workspace may be reused after each call. X, W, keep,

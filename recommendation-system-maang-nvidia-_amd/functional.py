@@ -1387,7 +1387,7 @@ class _on:
         self.prev = -1
 
     def __enter__(self):
-        cur = torch.cuda.current_device()
+        cur = torch._C._cuda_getDevice()
         if cur != self.index:
             self.prev = cur
             torch.cuda.set_device(self.index)
@@ -1408,10 +1408,11 @@ def _catalog_bytes(N, V, D, dt, want):
 class CatalogSoftmaxState:
     """What catalog_softmax_fwd hands to catalog_softmax_bwd: the operands' images, the rows'
     statistics and the unit gradient of X, in one buffer that the backward only reads."""
-    __slots__ = ("keep", "N", "V", "D", "dtype", "scale", "want")
+    __slots__ = ("keep", "N", "V", "D", "dtype", "scale", "want", "ws_bytes")
 
-    def __init__(self, keep, N, V, D, dtype, scale, want):
-        self.keep, self.N, self.V, self.D, self.dtype, self.scale, self.want = keep, N, V, D, dtype, scale, want
+    def __init__(self, keep, N, V, D, dtype, scale, want, ws_bytes):
+        self.keep, self.N, self.V, self.D, self.dtype = keep, N, V, D, dtype
+        self.scale, self.want, self.ws_bytes = scale, want, ws_bytes
 
 
 def _catalog_check(X, W, labels, weights, scale, reduction):
@@ -1445,6 +1446,11 @@ def catalog_softmax_fwd(X, W, labels, scale: float = 1.0, weights=None, ignore_i
     weights for reduction "mean" (0 without a labelled row); state is for catalog_softmax_bwd.
     want_grad: False (the loss alone, about half the work), True, or a pair (dX, dW) of bools.
     A label outside [0, V) that is not ignore_index makes its row and the loss NaN."""
+    return _catalog_fwd(X, W, labels, scale, weights, ignore_index, reduction, want_grad, True)
+
+
+def _catalog_fwd(X, W, labels, scale, weights, ignore_index, reduction, want_grad, want_lse):
+    """catalog_softmax_fwd, its lse optional (else None)"""
     scale, ignore_index = float(scale), int(ignore_index)
     _catalog_check(X, W, labels, weights, scale, reduction)
     want_x, want_w = want_grad if isinstance(want_grad, (tuple, list)) else (want_grad, want_grad)
@@ -1458,12 +1464,12 @@ def catalog_softmax_fwd(X, W, labels, scale: float = 1.0, weights=None, ignore_i
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
         loss = torch.empty((), dtype=torch.float32, device=dev)
         row = torch.empty(N, dtype=torch.float32, device=dev)
-        lse = torch.empty(N, dtype=torch.float32, device=dev)
+        lse = torch.empty(N, dtype=torch.float32, device=dev) if want_lse else None
         call("rs_catalog_softmax_fwd", X.data_ptr(), W.data_ptr(), labels.data_ptr(),
              weights.data_ptr() if weights is not None else None, N, V, D, dt, scale, ignore_index,
-             reduction == "mean", want, loss.data_ptr(), row.data_ptr(), lse.data_ptr(), keep.data_ptr(), keep_bytes,
-             ws.data_ptr(), ws_bytes, stream)
-    return loss, row, lse, CatalogSoftmaxState(keep, N, V, D, X.dtype, scale, want)
+             reduction == "mean", want, loss.data_ptr(), row.data_ptr(), lse.data_ptr() if want_lse else None,
+             keep.data_ptr(), keep_bytes, ws.data_ptr(), ws_bytes, stream)
+    return loss, row, lse, CatalogSoftmaxState(keep, N, V, D, X.dtype, scale, want, ws_bytes)
 
 
 def catalog_softmax_bwd(W, state: CatalogSoftmaxState, g=None, dx: bool = True, dw: bool = True):
@@ -1478,19 +1484,18 @@ def catalog_softmax_bwd(W, state: CatalogSoftmaxState, g=None, dx: bool = True, 
         raise ValueError("catalog_softmax_bwd: the forward was not asked for this gradient (want_grad)")
     if g is not None and (_dev(g, "g").numel() != 1 or g.device != dev):
         raise ValueError("catalog_softmax_bwd: g must be one float32 value on W's device")
-    return _catalog_bwd(_aligned(W), state, g, dx, dw)
+    return _catalog_bwd(_aligned(W), state.keep, state, g, dx, dw)
 
 
-def _catalog_bwd(W, state, g, dx, dw):
-    N, V, D, dt, dev = state.N, state.V, state.D, RS_DTYPES[state.dtype], state.keep.device
-    ws_bytes = _catalog_bytes(N, V, D, dt, state.want)[1]
+def _catalog_bwd(W, keep, state, g, dx, dw):
+    N, V, D, ty, dev = state.N, state.V, state.D, state.dtype, keep.device
     with _on(W) as stream:
-        dX = torch.empty((N, D), dtype=state.dtype, device=dev) if dx else None
-        dW = torch.empty((V, D), dtype=state.dtype, device=dev) if dw else None
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-        call("rs_catalog_softmax_bwd", W.data_ptr(), N, V, D, dt, state.scale, state.want,
-             g.data_ptr() if g is not None else None, state.keep.data_ptr(), state.keep.numel(),
-             dX.data_ptr() if dx else None, dW.data_ptr() if dw else None, ws.data_ptr(), ws_bytes, stream)
+        dX = torch.empty((N, D), dtype=ty, device=dev) if dx else None
+        dW = torch.empty((V, D), dtype=ty, device=dev) if dw else None
+        ws = torch.empty(state.ws_bytes, dtype=torch.uint8, device=dev)
+        call("rs_catalog_softmax_bwd", W.data_ptr(), N, V, D, RS_DTYPES[ty], state.scale, state.want,
+             g.data_ptr() if g is not None else None, keep.data_ptr(), keep.numel(), dX.data_ptr() if dx else None,
+             dW.data_ptr() if dw else None, ws.data_ptr(), state.ws_bytes, stream)
     return dX, dW
 
 
@@ -2376,11 +2381,11 @@ class CatalogSoftmaxFn(torch.autograd.Function):
     def forward(ctx, X, W, labels, weights, scale: float, ignore_index: int, reduction: str):
         ctx.set_materialize_grads(False)
         W = W.contiguous()
-        loss, row, _, st = catalog_softmax_fwd(
+        loss, row, _, st = _catalog_fwd(
             X.contiguous(), W, labels.contiguous(), scale, weights.contiguous() if weights is not None else None,
-            ignore_index, reduction, want_grad=(ctx.needs_input_grad[0], ctx.needs_input_grad[1]))
-        ctx.save_for_backward(W, st.keep)   # (the state's buffer goes with the saved tensors)
-        ctx.sizes = st.N, st.V, st.D, st.dtype, st.scale, st.want
+            ignore_index, reduction, ctx.needs_input_grad[:2], False)
+        ctx.save_for_backward(W, st.keep)   # (the state's buffer is freed with the saved tensors)
+        st.keep, ctx.state = None, st
         ctx.mark_non_differentiable(row)
         return loss, row
 
@@ -2390,8 +2395,7 @@ class CatalogSoftmaxFn(torch.autograd.Function):
         if g is None:
             return (None,) * 7
         W, keep = ctx.saved_tensors
-        dX, dW = _catalog_bwd(_aligned(W), CatalogSoftmaxState(keep, *ctx.sizes), g.contiguous(),
-                              ctx.needs_input_grad[0], ctx.needs_input_grad[1])
+        dX, dW = _catalog_bwd(_aligned(W), keep, ctx.state, g, *ctx.needs_input_grad[:2])
         return dX, dW, None, None, None, None, None
 
 
@@ -2400,9 +2404,9 @@ def catalog_softmax_loss(X, W, labels, scale: float = 1.0, weights=None, ignore_
     """(loss, row_loss) of catalog_softmax_fwd, differentiable by X and W through the loss (not by the
     weights). With gradients disabled the loss alone is formed (want_grad=False)."""
     if not torch.is_grad_enabled():   # (a node is not told: its needs_input_grad are the inputs' requires_grad)
-        return catalog_softmax_fwd(X.contiguous(), W.contiguous(), labels.contiguous(), scale,
-                                   weights.contiguous() if weights is not None else None, ignore_index, reduction,
-                                   want_grad=False)[:2]
+        return _catalog_fwd(X.contiguous(), W.contiguous(), labels.contiguous(), scale,
+                            weights.contiguous() if weights is not None else None, ignore_index, reduction,
+                            False, False)[:2]
     if weights is not None and weights.requires_grad:
         raise ValueError("catalog_softmax_loss: the loss is not differentiable by its weights; detach them")
     return CatalogSoftmaxFn.apply(X, W, labels, weights, scale, ignore_index, reduction)

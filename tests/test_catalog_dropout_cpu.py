@@ -29,7 +29,8 @@ def test_cpu_tensors_are_refused():
 @pytest.mark.parametrize("bad,match", [
     (dict(N=-1), "bad sizes"), (dict(V=0), "bad sizes"), (dict(D=0), "bad sizes"), (dict(N=1 << 26), "2\\^26"),
     (dict(V=1 << 29), "2\\^29"), (dict(N=1 << 25, D=256), "2\\^33"), (dict(D=257), "above 256"),
-    (dict(dtype=7), "dtype"), (dict(scale=0.0), "scale"), (dict(scale=float("nan")), "scale"), (dict(want=4), "flags"), (dict(x=None), "null"), (dict(w=None), "null"),
+    (dict(dtype=7), "dtype"), (dict(scale=0.0), "scale"), (dict(scale=float("nan")), "scale"),
+    (dict(want=4), "flags"), (dict(x=None), "null"), (dict(w=None), "null"),
     (dict(labels=None), "null"), (dict(x=A + 4), "aligned"), (dict(w=A + 8), "aligned"), (dict(keep=64), "keep"),
     (dict(ws=64), "workspace")])
 def test_forward_refusals(bad, match):
@@ -88,13 +89,12 @@ def test_the_loss_alone_without_gradients(monkeypatch):
     F = pkg("functional")
     asked = []
 
-    def fwd(X, W, labels, scale=1.0, weights=None, ignore_index=-100, reduction="sum", want_grad=True):
+    def fwd(X, W, labels, scale, weights, ignore_index, reduction, want_grad, want_lse):
         asked.append(want_grad)
-        z = torch.zeros(())
-        keep = torch.empty(1)
-        return z, torch.zeros(X.shape[0]), None, F.CatalogSoftmaxState(keep, *X.shape, W.shape[0], X.dtype, scale, 0)
+        st = F.CatalogSoftmaxState(torch.empty(1), X.shape[0], W.shape[0], X.shape[1], X.dtype, scale, 0, 256)
+        return torch.zeros(()), torch.zeros(X.shape[0]), None, st
 
-    monkeypatch.setattr(F, "catalog_softmax_fwd", fwd)
+    monkeypatch.setattr(F, "_catalog_fwd", fwd)
     x, w = torch.zeros((3, 8)), torch.zeros((5, 8), requires_grad=True)
     y = torch.zeros(3, dtype=torch.int64)
     loss, _ = F.catalog_softmax_loss(x, w, y)
