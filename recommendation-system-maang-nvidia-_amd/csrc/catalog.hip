@@ -911,7 +911,7 @@ struct CsRows {
   float scale, kbase;
   float *row, *lse, *dx, *stat;
   CsScal* scal;
-  unsigned int* done;  // completion tickets (ticket_last)
+  unsigned int* done;  // completion tickets (ticket_last), or null: the total is another kernel's
   int mean;
   float* loss;
 };
@@ -919,24 +919,34 @@ __device__ __forceinline__ float cs_ld(const void* x, int bf16, int64_t i) {
   return bf16 ? (float)((const __bf16*)x)[i] : ((const float*)x)[i];
 }
 
-// the loss, 1 / Z and whether a weight is negative: one workgroup of at most 512 threads, fixed order. The
-// row losses may come from other workgroups of the same grid.
+// the loss, 1 / Z and whether a weight is negative: one workgroup, fixed order. The row losses may come
+// from other workgroups of the same grid.
 __device__ __forceinline__ void cs_total(const CsRows& p) {
-  __shared__ double sh[2][8];
+  __shared__ double sh[2][16];
   __shared__ int neg;
   const int threads = blockDim.x, waves = threads / 64;
   if (threadIdx.x == 0) neg = 0;
   __syncthreads();
   double s = 0., z = 0.;
   bool below = false;
-#pragma unroll 8
-  for (int64_t n = threadIdx.x; n < p.N; n += threads) {
-    const bool in = p.lab[n] != -1;
-    const float a = p.weights ? p.weights[n] : 1.f;
-    const float r = __hip_atomic_load(p.row + n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    below |= in && a < 0.f;
-    s += in ? (double)a * (double)r : 0.;
-    z += in ? (double)a : 0.;
+  constexpr int U = 8;  // loads in flight
+  for (int64_t n0 = threadIdx.x; n0 < p.N; n0 += U * threads) {
+    float r[U], a[U];
+    int32_t lab[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t n = n0 + u * threads, i = n < p.N ? n : p.N - 1;
+      r[u] = __hip_atomic_load(p.row + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      a[u] = p.weights ? p.weights[i] : 1.f;
+      lab[u] = n < p.N ? p.lab[i] : -1;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool in = lab[u] != -1;
+      below |= in && a[u] < 0.f;
+      s += in ? (double)a[u] * (double)r[u] : 0.;
+      z += in ? (double)a[u] : 0.;
+    }
   }
   if (below) neg = 1;
   s = wave_sum_d(s);
@@ -958,7 +968,7 @@ __device__ __forceinline__ void cs_total(const CsRows& p) {
     *p.loss = (float)(s * inv);
   }
 }
-__global__ __launch_bounds__(64) void cs_no_rows_kernel(CsRows p) { cs_total(p); }
+__global__ __launch_bounds__(1024) void cs_total_kernel(CsRows p) { cs_total(p); }
 
 // Joins the splits of a row: NWV waves per row (1: four rows per workgroup), DP / 4 lanes per split, the
 // splits dealt to the lane groups and their sums joined in a fixed order. Then the label's logit (64-bit
@@ -1063,11 +1073,14 @@ __device__ __forceinline__ void cs_row(const CsRows& p) {
   }
 }
 
-// The rows, and in the grid's last workgroup the total: 4 to 6 us more than the rows alone where a kernel of
-// its own took 4 and a launch (20 and 11 at 16384 rows of 14 ms).
+// The rows, and up to CS_TAIL_ROWS of them the total in the grid's last workgroup: 3 to 6 us more than the
+// rows alone, a kernel of its own 4 to 5 and a launch of the host's time, which bounds such a step. Past
+// that the tickets cost more (4096 rows: 22 us against 13 + 5; 8192: 27 against 16 + 7).
+constexpr int CS_TAIL_ROWS = 2048;
 template <int DP, int NP, int NWV>
 __global__ __launch_bounds__(NWV == 1 ? 256 : 64 * NWV) void cs_rows_kernel(CsRows p) {
   cs_row<DP, NP, NWV>(p);
+  if (!p.done) return;
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's row losses are out
   __syncthreads();
   if (ticket_last(p.done, blockIdx.x, gridDim.x)) cs_total(p);
@@ -1369,7 +1382,8 @@ extern "C" int rs_catalog_softmax_fwd(const void* X, const void* W, const int64_
     else cs_launch_pass<CS_STATS>(s, p, s.rnrb * s.rsplit, st);
   }
   const CsRows r{X, W, s.NP == 1, N, s.Npad, V, D, s.rsplit, w.m, w.l, w.O, k.lab, weights, k.kx, scale, kbase, row_loss,
-                 lse, k.dx, want & RS_CATALOG_DW ? k.stat : nullptr, k.scal, w.done, mean, loss};
+                 lse, k.dx, want & RS_CATALOG_DW ? k.stat : nullptr, k.scal,
+                 N <= CS_TAIL_ROWS ? w.done : nullptr, mean, loss};
   if (N > 0) {
     // many splits of few rows: a workgroup per row, else a wave
     const int wide = s.rsplit > 64 ? 8 : s.rsplit > 8 ? 4 : 0;
@@ -1383,7 +1397,7 @@ extern "C" int rs_catalog_softmax_fwd(const void* X, const void* W, const int64_
     CS_GO(64, 1) CS_GO(64, 2) CS_GO(128, 1) CS_GO(128, 2) CS_GO(256, 1) CS_GO(256, 2)
 #undef CS_GO
   }
-  if (N == 0) hipLaunchKernelGGL(cs_no_rows_kernel, dim3(1), dim3(64), 0, st, r);
+  if (N == 0 || !r.done) hipLaunchKernelGGL(cs_total_kernel, dim3(1), dim3(1024), 0, st, r);
   return check_launch("catalog_softmax_fwd");
 }
 

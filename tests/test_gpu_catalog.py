@@ -111,7 +111,8 @@ def test_against_float64(cuda, dtype, N, V, D):
 
 @DTYPES
 @pytest.mark.parametrize("reduction", ["sum", "mean"])
-@pytest.mark.parametrize("N,V,D,scale", [(300, 500, 64, 1 / 0.07), (97, 2500, 128, 0.25), (260, 300, 200, 1.0)])
+@pytest.mark.parametrize("N,V,D,scale", [(300, 500, 64, 1 / 0.07), (97, 2500, 128, 0.25), (260, 300, 200, 1.0),
+                                         (2048, 60, 64, 0.5), (2049, 300, 128, 0.5), (9000, 40, 64, 1.0)])
 def test_weights_ignored_scale(cuda, dtype, reduction, N, V, D, scale):
     x, w, y, a = inputs(N, V, D, dtype, seed=7, ignored=0.4, weights=True, scale=scale)
     check(x, w, y, a, scale, reduction, g=-2.5)
