@@ -26,9 +26,9 @@
 // is formed in fresh accumulators and added in fp32 (the matrix unit's long running sums lose bits).
 //
 // Bound: the matrix cores' rate at the clock their load leaves (1.9 to 2.1 GHz; 54 to 63 % of the cycles
-// busy), the exponentials' vector work beside them. 16384 x 1M x 128 bf16, a training step: 13.4 ms, 1.25
-// PFLOP/s of its 8 N V D flops (a large bf16 library product: 1.16); 8192 x 100k x 128 fp32: 2.0 ms, 420
-// TFLOP/s, three fp16 products each (a large fp32 library product: 0.154 PFLOP/s). Fewer than ~300 rows:
+// busy), the exponentials' vector work beside them. 16384 x 1M x 128 bf16, a training step: 13.4 to 14.0 ms,
+// 1.20 to 1.25 PFLOP/s of its 8 N V D flops (a large bf16 library product: 1.16); 8192 x 100k x 128 fp32:
+// 2.0 ms, 420 TFLOP/s, three fp16 products each (a large fp32 library product: 0.154 PFLOP/s). Fewer than ~300 rows:
 // the catalogue's bytes.
 #include "split.hpp"
 
