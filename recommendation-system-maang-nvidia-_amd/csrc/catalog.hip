@@ -124,6 +124,13 @@ __device__ __forceinline__ int cs_exp2_split(float m, float& frac) {
   return (int)i;
 }
 
+// a pair of bf16, those that are not finite replaced by the largest number of their sign
+__device__ __forceinline__ uint32_t cs_finite_bf16(uint32_t w) {
+  if ((w & 0x7f80u) == 0x7f80u) w = (w & 0xffff8000u) | 0x7f7fu;
+  if ((w & 0x7f800000u) == 0x7f800000u) w = (w & 0x8000ffffu) | 0x7f7f0000u;
+  return w;
+}
+
 template <typename T>
 __device__ __forceinline__ T cs_lds(uint32_t off) {
   return *reinterpret_cast<__attribute__((address_space(3))) const T*>(off);
@@ -264,6 +271,13 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
       for (int pl = 0; pl < NP; ++pl)
         xq[ub][c][pl] = *reinterpret_cast<const u32x4*>(
             4 * c + g < p.r_ch ? p.R + pl * p.r_plane + q * p.r_ld + (4 * c + g) * 16 : p.zero);
+    // bf16: an infinite item becomes the largest finite one. Its probabilities are zero (or NaN, by the row's lse)
+    // either way, but the zeros of a row that takes no part stay zeros.
+    if constexpr (MODE == CS_COL && NP == 1)
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) xq[ub][c][0][j] = cs_finite_bf16(xq[ub][c][0][j]);
     if constexpr (MODE != CS_COL) {
       // FLT_MIN: a masked item's -inf must stay -inf after the product
       kq[ub] = NP == 2 ? fminf(fmaxf(p.kbase * p.scal->w_inv * p.kx[q], FLT_MIN), FLT_MAX) : p.kbase;
@@ -910,6 +924,7 @@ struct CsRows {
   const float* kx;
   float scale, kbase;
   float *row, *lse, *dx, *stat;
+  char* ximg;
   CsScal* scal;
   unsigned int* done;  // completion tickets (ticket_last), or null: the total is another kernel's
   int mean;
@@ -1061,6 +1076,9 @@ __device__ __forceinline__ void cs_row(const CsRows& p) {
     reinterpret_cast<int32_t*>(p.stat)[cs_stat(n, CS_LAB)] = live ? 2 * lb + (a < 0.f) : lb;
     p.stat[cs_stat(n, CS_LQ)] = (float)(o2 - lse2 + ca);
   }
+  // bf16: a row that takes no part is zero for the column pass, whose scores of it could pass fp32's range (the infinite
+  // statistic takes a finite score out, not an infinite one; fp32's scores are of scaled values)
+  if (NP == 1 && p.stat && lb < 0 && lane < LPR) *reinterpret_cast<u32x2*>(p.ximg + n * (2 * DP) + 2 * c) = u32x2{0, 0};
   if (!p.dx || lane >= LPR) return;
   const float il = L == 0. ? 0.f : (float)((NP == 2 ? (double)p.scal->w_inv : 1.) / L);
 #pragma unroll
@@ -1382,7 +1400,7 @@ extern "C" int rs_catalog_softmax_fwd(const void* X, const void* W, const int64_
     else cs_launch_pass<CS_STATS>(s, p, s.rnrb * s.rsplit, st);
   }
   const CsRows r{X, W, s.NP == 1, N, s.Npad, V, D, s.rsplit, w.m, w.l, w.O, k.lab, weights, k.kx, scale, kbase, row_loss,
-                 lse, k.dx, want & RS_CATALOG_DW ? k.stat : nullptr, k.scal,
+                 lse, k.dx, want & RS_CATALOG_DW ? k.stat : nullptr, k.ximg, k.scal,
                  N <= CS_TAIL_ROWS ? w.done : nullptr, mean, loss};
   if (N > 0) {
     // many splits of few rows: a workgroup per row, else a wave

@@ -1,0 +1,67 @@
+"""The catalogue softmax where rows or items hold values far from the others': rows that take no part,
+masked items, items of different scales. Reference and tolerances are test_gpu_catalog's."""
+import pytest
+import torch
+
+from conftest import pkg
+from test_gpu_catalog import DTYPES, IGN, inputs, reference, step, tolerances, within
+
+pytestmark = pytest.mark.gpu
+
+
+@DTYPES
+@pytest.mark.parametrize("N", [200, 2049])
+@pytest.mark.parametrize("D", [64, 96, 256])
+def test_excluded_rows_may_hold_the_largest_values(cuda, dtype, N, D):
+    """Ignored rows, and rows whose label is out of range, reach no item's gradient, whatever finite values
+    they hold: their logits pass the type's range."""
+    x, w, y, _ = inputs(N, 300, D, dtype, seed=3, ignored=0.3)
+    w = (w.float() * 4).to(dtype)
+    y[13], y[77] = 300, -1
+    dead = (y == IGN) | (y < 0) | (y >= 300)
+    clean = torch.where(dead, torch.full_like(y, IGN), y)
+    x2 = x.clone()
+    g = torch.Generator().manual_seed(1)
+    sign = torch.randint(0, 2, x.shape, generator=g).cuda() * 2 - 1
+    x2[dead] = (sign * torch.finfo(dtype).max).to(dtype)[dead]
+    _, row, dx, dw = step(x, w, clean)
+    _, row2, dx2, dw2 = step(x2, w, y)
+    assert torch.equal(row[~dead], row2[~dead]) and torch.equal(dx[~dead], dx2[~dead]) and torch.equal(dw, dw2)
+
+
+def masked(N, V, D, dtype, bias, seed=0):
+    """x's last column is 1, w's the item's bias; every seventh item is masked by it. Ignored rows are
+    zeros, as a padded batch has them. Labels are items that are not masked."""
+    x, w, y, _ = inputs(N, V, D, dtype, seed=seed, ignored=0.2)
+    x[:, -1] = 1.0
+    x[y == IGN] = 0.0
+    gone = torch.arange(V, device="cuda") % 7 == 3
+    w[:, -1] = torch.where(gone, torch.full_like(w[:, -1], bias), 0.25 * w[:, -1])
+    y = torch.where(y == IGN, y, torch.where(gone[y.clamp(min=0)], y.clamp(min=0) + 1, y) % V)
+    return x, w, y, gone
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16], ids=["bf16"])
+@pytest.mark.parametrize("bias", [-1e4, -1e9, -1e30, -float("inf")])
+@pytest.mark.parametrize("N,V,D", [(40, 500, 64), (64, 701, 96), (65, 701, 100), (130, 1000, 128), (300, 259, 256)])
+def test_masked_items(cuda, dtype, bias, N, V, D):
+    """A masked item changes no other item's logit: loss and gradients are those of the catalogue without it,
+    its own gradient is zero. (With an infinite bias the formula has no value in dX's column of the biases.)"""
+    F = pkg("functional")
+    x, w, y, gone = masked(N, V, D, dtype, bias, seed=N + V)
+    at = torch.cumsum(~gone, 0) - 1                      # an item's row among those that are left
+    wk, yk = w[~gone], torch.where(y == IGN, y, at[y.clamp(min=0)])
+    r = reference(x, wk, yk, 1.0, None, "mean")
+    t = tolerances(r, N, V, D, dtype)
+    loss, row, dx, dw = step(x, w, y, reduction="mean")
+    l2, row2, lse, _ = F.catalog_softmax_fwd(x, w, y, 1.0, None, IGN, "mean", want_grad=False)
+    within(row, r["row"], t["row"], "row")
+    within(row2, r["row"], t["row"], "row (loss alone)")
+    within(loss, r["loss"], t["loss"], "loss")
+    within(l2, r["loss"], t["loss"], "loss alone")
+    live = (y != IGN).cpu()
+    within(lse.cpu()[live], r["lse"][live], t["row"][live], "lse")
+    within(dw[~gone], r["dw"], t["dw"], "dw")
+    assert not bool(dw[gone].any())
+    cols = D - 1 if bias == -float("inf") else D
+    within(dx[:, :cols], r["dx"][:, :cols], t["dx"][:, :cols], "dx")
