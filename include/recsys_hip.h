@@ -813,7 +813,12 @@ int rs_l2_normalize_rows_f32(const float* x, int64_t n, int64_t D, float* out, r
  *   s_nv = c <x_n, w_v>, lse_n = log sum_v exp s_nv, row_n = lse_n - s_n,label, loss = sum a_n row_n / Z,
  * Z = 1, or with `mean` the sum of a over the labelled rows (a sum of zero, or no labelled row: loss 0).
  * No logits are
- * stored. An ignored row has row_loss 0, enters neither loss nor gradients (whatever its x holds) and
+ * stored. float32 operands are held as two fp16 terms under a power-of-two scale for each row of X and each
+ * item: a logit's error is at most c (2^-20 sum_d |x_d w_d| + D 2^-30 max|x_n| max|w_v|) beside fp32 sums.
+ * bfloat16 operands are exact; the gradients' probabilities are rounded to bfloat16. An item is masked by a
+ * logit far below the others or of -infinity (one infinite entry of w against a finite one of x): the rest is
+ * as without it, its row of dW zero; dX's column of an infinite entry has no value. A NaN entry, or a logit of
+ * +infinity, makes its rows NaN. Where every logit of a row lies below -1e30 its loss has no value. An ignored row has row_loss 0, enters neither loss nor gradients (whatever its x holds) and
  * has the lse of its finite entries; a label that is neither in range nor ignore_index makes its row
  * loss, its dX row and the loss NaN and stays out of dW. row_loss, lse [N] (nullable) and *loss are fp32.
  * want: RS_CATALOG_DX / _DW: which gradients a backward will be asked for (0: the loss alone, about

@@ -20,10 +20,12 @@
 // bf16 inputs: one bf16 product, p rounded to bf16 (2^-8 of each term, as its output is). fp32 inputs:
 // every operand as two fp16 terms h + l of the value scaled by a power of two (|x - h - l| <= 2^-22
 // |x|, or 2^-39 of the scale's largest value), three products h h, h l, l h per fp32 product: half the
-// matrix work of the exact three-term bf16 split, rounding below an fp32 dot product's own. Rows of x
-// have a scale each; w, which the row pass sums over, has one. p is scaled against the running maximum
-// (kept in both passes) so that unlikely items keep their relative precision, and each tile's sum
-// is formed in fresh accumulators and added in fp32 (the matrix unit's long running sums lose bits).
+// matrix work of the exact three-term bf16 split. Every row of x and every item has a scale of its own, so
+// an item takes no bits from another. A logit's error is c sum_d |x_d w_d| 2^-20, like an fp32 product's own
+// rounding, plus c D 2^-30 max|x_n| max|w_v|: more than that only where an entry 2^10 and more below its item's
+// largest one meets an x that makes up for it. In both passes P carries the streamed row's scale and is itself scaled against a running maximum of
+// the scaled terms, so that unlikely or small items keep their relative precision, and each tile's sum is
+// formed in fresh accumulators and added in fp32 (the matrix unit's long running sums lose bits).
 //
 // Bound: the matrix cores' rate at the clock their load leaves (1.9 to 2.1 GHz; 54 to 63 % of the cycles
 // busy), the exponentials' vector work beside them. 16384 x 1M x 128 bf16, a training step: 13.4 to 14.0 ms,
@@ -43,16 +45,14 @@ typedef _Float16 cs_h2 __attribute__((ext_vector_type(2)));
 
 constexpr float CS_MIN = -1e30f;     // the running maximum before any item
 constexpr float CS_PS = 15.f;        // fp16 exponentials are formed at 2^15 (below 65504)
-constexpr int CS_AMAX_BLOCKS = 512;  // partial maxima of |w|
 constexpr double CS_LOG2E = 1.4426950408889634074;
 constexpr double CS_LN2 = 0.69314718055994530942;
 
 // device scalars of a call (in the kept buffer)
 struct CsScal {
-  float w_inv;   // 2^-e of the catalogue's scale (fp32), 1 (bf16)
   float inv_z;   // 1 / Z of the reduction
   int32_t neg;   // a labelled row's weight is negative
-  float pad;
+  float pad[2];
   float zero[4];  // 16 zero bytes, for the columns past a width
 };
 
@@ -64,6 +64,17 @@ struct CsScal {
 enum { CS_LSE2 = 0, CS_KX = 1, CS_LAB = 2, CS_LQ = 3 };
 constexpr int CS_XREF = 13;
 __host__ __device__ inline int64_t cs_stat(int64_t n, int a) { return (n >> 5) * 128 + a * 32 + (n & 31); }
+
+// fp32: an item's scale 2^e, per 32 items two arrays of 32 words: f = 2^(-e - 1), the factor of its scores and
+// of its exponentials in the row pass's second product, and -log2 f. e = 3 + 8 i brings the item's largest entry
+// into [2^6, 2^14) (i = 1: entries from 2^-5 to 2^3): neighbours mostly share it, and what they share costs no work
+// per score (row pass of 4096 x 20k x 64: 95 us with one scale, 103 with items over 16 binades; 8192 x 100k x 128: 0.98
+// ms and 0.99). An item with an entry that is not finite has 2^90 and infinity (NaN, if one of them is), and +-2^14
+// for its infinite entries, zeros for the others. e is at most 99 (2^-27 for the smallest normal number): an
+// exponential in the row pass stays between 2^-101 (the row's likeliest item) and 2^115.
+enum { CS_WF = 0, CS_WE = 1 };
+constexpr int CS_WE_MAX = 99;
+__host__ __device__ inline int64_t cs_wstat(int64_t v, int a) { return (v >> 5) * 64 + a * 32 + (v & 31); }
 
 struct CsPass {
   const char* R;          // resident rows [nR][D] (plane stride r_plane bytes)
@@ -77,11 +88,12 @@ struct CsPass {
   int full, nsplit, nrb;  // the first `full` resident blocks are not split, the other nrb are
   const CsScal* scal;
   float scale, kbase;     // c, c log2 e
-  const float* kx;        // row pass, fp32: 2^-e of each resident row
+  const float* kr;        // fp32: factors of the resident rows (row pass: 2^-e of x's rows, column pass: w's statistics)
   const int32_t* lab;     // row pass: label of each resident row (< 0: none)
-  const float* stat;      // column pass: statistics of the streamed rows
+  const float* stat;      // statistics of the streamed rows (column pass; fp32's row pass)
   int64_t pR;             // rows of the partials: those of the split blocks (full = 0: all, split or not)
-  float *m, *l, *O;       // partials m, l [pR][split], O [split][pR][D]
+  float *m, *O;           // partials m, l [pR][split], O [split][pR][D]
+  double* l;
   // column pass: the gradient of the unsplit blocks
   void* out;
   int64_t ld;             // its row length
@@ -116,12 +128,31 @@ __device__ __forceinline__ void cs_glds16(const char* g, uint32_t dst) {
                : "memory");
 }
 
+// the same from a uniform address plus 16 lane
+__device__ __forceinline__ void cs_glds16u(const char* g, int lane, uint32_t dst) {
+  const uint32_t m0v = __builtin_amdgcn_readfirstlane(dst);
+  uint32_t keep;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
+               : "=&s"(keep)
+               : "v"(16 * lane), "s"(g), "s"(m0v)
+               : "memory");
+}
+
 // 2^m, an integer exponent (for ldexp) apart from a factor of one binade: an item that no row expects has
 // an m far below the smallest number while its gradient is none of these
 __device__ __forceinline__ int cs_exp2_split(float m, float& frac) {
   const float i = fmaxf(floorf(m), -1000.f);
   frac = __builtin_amdgcn_exp2f(fmaxf(m, -1000.f) - i);
   return (int)i;
+}
+
+// 2^d of a difference of two maxima, d <= 0. fp32's maxima are of scaled terms: 2^d may be below the smallest fp32 number
+// where the sum it multiplies is far above one
+template <int NP>
+__device__ __forceinline__ double cs_exp2_d(float d) {
+  if (NP == 1) return (double)__builtin_amdgcn_exp2f(d);
+  const double h = (double)__builtin_amdgcn_exp2f(0.5f * d);
+  return h * h;
 }
 
 // a pair of bf16, those that are not finite replaced by the largest number of their sign
@@ -201,7 +232,8 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
   constexpr int UB = cs_cfg(D, NP, MODE).UB, NW = cs_cfg(D, NP, MODE).NW, KT = cs_cfg(D, NP, MODE).KT;
   constexpr int NB = cs_cfg(D, NP, MODE).NB;
   constexpr int ROWB = 2 * D, PLANE = KT * ROWB, IMG = NP * PLANE, NDT = D / 16, NC = D / 32;
-  constexpr int STAT = MODE == CS_COL ? KT * 16 : 0, BUF = IMG + STAT;
+  constexpr int SROW = MODE == CS_COL ? 16 : NP == 2 ? 8 : 0;  // bytes of statistics per streamed row
+  constexpr int STAT = KT * SROW, BUF = IMG + STAT;
   constexpr bool RUNMAX = MODE != CS_COL || NP == 2;
   __shared__ __attribute__((aligned(1024))) char smem[NB * BUF];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -249,9 +281,11 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
         cs_glds16(q + pl * p.t_plane, lds0 + buf * BUF + pl * PLANE + i * NW * 1024 + wave * 1024);
       src[i] += src_step[i];
     }
-    if constexpr (MODE == CS_COL)
-      if (wave == 0 && lane < KT)
-        cs_glds16((const char*)p.stat + t * (KT * 16) + lane * 16, lds0 + buf * BUF + IMG);
+    if constexpr (SROW > 0)
+      if (wave == 0 && lane < STAT / 16) {
+        if constexpr (NP == 2) cs_glds16u((const char*)p.stat + t * STAT, lane, lds0 + buf * BUF + IMG);
+        else cs_glds16((const char*)p.stat + t * STAT + lane * 16, lds0 + buf * BUF + IMG);
+      }
   };
 #pragma unroll
   for (int i = 0; i < AHEAD; ++i)
@@ -280,8 +314,10 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
         for (int j = 0; j < 4; ++j) xq[ub][c][0][j] = cs_finite_bf16(xq[ub][c][0][j]);
     if constexpr (MODE != CS_COL) {
       // FLT_MIN: a masked item's -inf must stay -inf after the product
-      kq[ub] = NP == 2 ? fminf(fmaxf(p.kbase * p.scal->w_inv * p.kx[q], FLT_MIN), FLT_MAX) : p.kbase;
+      kq[ub] = NP == 2 ? fminf(fmaxf(2.f * p.kbase * p.kr[q], FLT_MIN), FLT_MAX) : p.kbase;
       lab[ub] = p.lab[q];
+    } else if constexpr (NP == 2) {
+      kq[ub] = p.kr[cs_wstat(q, CS_WF)];
     }
   }
   // the resident rows are waited for here: a wait inside the loop would also wait for every copy in flight
@@ -292,18 +328,30 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
 #pragma unroll
       for (int pl = 0; pl < NP; ++pl) asm volatile("" : "+v"(xq[ub][c][pl]));
     if constexpr (MODE != CS_COL) asm volatile("" : "+v"(kq[ub]), "+v"(lab[ub]));
+    else if constexpr (NP == 2) asm volatile("" : "+v"(kq[ub]));
+  }
+  // fp32's column pass: the wave's items share a scale, or have one each (kq)
+  bool same = true;
+  float f0 = 1.f;
+  if constexpr (MODE == CS_COL && NP == 2) {
+    f0 = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, kq[0])));
+#pragma unroll
+    for (int ub = 0; ub < UB; ++ub) same &= !__any(kq[ub] != f0);
   }
   const float kw = p.kbase;
   const float ps = NP == 2 ? CS_PS : 0.f;
   const bool flip = MODE == CS_COL && p.scal->neg;
 
   // row reads: A row i16 of subtile kb = row 8 (i16 / 4) + 4 kb + i16 % 4 of 32, chunk 4 c + g
-  const uint32_t ab = lds0 + (i16 >> 2) * (8 * ROWB) + (i16 & 3) * 64 + (g ^ cs_swz(i16 >> 2)) * 16;
-  // transposed reads: row 8 g + 4 h + i16 / 4 of 32, columns 16 dt + 4 (i16 % 4) .., by dt % 2
-  uint32_t tb[2];
-#pragma unroll
-  for (int o = 0; o < 2; ++o)
-    tb[o] = lds0 + g * (8 * ROWB) + (i16 >> 2) * 64 + ((2 * o + ((i16 & 3) >> 1)) ^ cs_swz(g)) * 16 + 8 * (i16 & 1);
+  auto row_at = [&](int ln) __attribute__((always_inline)) {
+    const int g = ln >> 4, i16 = ln & 15;
+    return lds0 + (i16 >> 2) * (8 * ROWB) + (i16 & 3) * 64 + (g ^ cs_swz(i16 >> 2)) * 16;
+  };
+  // transposed reads: row 8 g + 4 h + i16 / 4 of 32, columns 16 dt + 4 (i16 % 4) .., by o = dt % 2
+  auto col_at = [&](int ln, int o) __attribute__((always_inline)) {
+    const int g = ln >> 4, i16 = ln & 15;
+    return lds0 + g * (8 * ROWB) + (i16 >> 2) * 64 + ((2 * o + ((i16 & 3) >> 1)) ^ cs_swz(g)) * 16 + 8 * (i16 & 1);
+  };
 
   f32x4 O[MODE == CS_STATS ? 1 : NDT][UB];
 #pragma unroll
@@ -325,8 +373,8 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
   };
 
   // S of the group's streamed rows at LDS byte bo, one step = 32 columns of 32 rows
-  auto scores = [&](uint32_t bo, Scores& s) __attribute__((always_inline)) {
-    uint32_t at = ab + bo;
+  auto scores = [&](int ln, uint32_t bo, Scores& s) __attribute__((always_inline)) {
+    uint32_t at = row_at(ln) + bo;
     asm("" : "+v"(at));  // the offsets below stay in the instructions
     constexpr int NST = SG * NC, AH = cs_ahead(NP, CS_S);
     u32x4 a[AH + 1][2][NP];
@@ -361,8 +409,8 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
   };
   // O += P times the group's rows. fp32 operands: the group's sum in fresh accumulators, then one fp32
   // multiply-add that also brings O to the scale P was formed at.
-  auto product = [&](uint32_t bo, const Probs& pb, const float (&al)[UB]) __attribute__((always_inline)) {
-    uint32_t at[2] = {tb[0] + bo, tb[1] + bo};
+  auto product = [&](int ln, uint32_t bo, const Probs& pb, const float (&al)[UB]) __attribute__((always_inline)) {
+    uint32_t at[2] = {col_at(ln, 0) + bo, NP == 2 ? (col_at(ln, 0) + bo) ^ 32 : col_at(ln, 1) + bo};  // (o is bit 5)
     asm("" : "+v"(at[0]), "+v"(at[1]));
     constexpr int NST = SG * NDT, AH = cs_ahead(NP, CS_P);
     u32x4 a[AH + 1][NP];
@@ -402,14 +450,22 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
       __builtin_amdgcn_sched_barrier(0);
     }
   };
-  // four probabilities of subtile k -> words of P
-  auto pack = [&](Probs& pb, int k, int ub, f32x4 e) __attribute__((always_inline)) {
+  // four probabilities of subtile k -> words of P (fp32's row pass: times the items' factors f, the products
+  // part of the two roundings)
+  auto pack = [&](Probs& pb, int k, int ub, f32x4 e, f32x4 f) __attribute__((always_inline)) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const float a = e[2 * h], b = e[2 * h + 1];
       const int w = 2 * (k & 1) + h;
       if constexpr (NP == 1) pb.w[k >> 1][ub][0][w] = ib_pk(a, b);
-      else {
+      else if constexpr (MODE == CS_ROW) {
+        const float fa = f[2 * h], fb = f[2 * h + 1];
+        const cs_h2 hi = __builtin_bit_cast(cs_h2, __builtin_amdgcn_cvt_pkrtz(a * fa, b * fb));
+        pb.w[k >> 1][ub][0][w] = __builtin_bit_cast(uint32_t, hi);
+        pb.w[k >> 1][ub][1][w] =
+            __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf(a, fa, -(float)hi[0]),
+                                                                    __builtin_fmaf(b, fb, -(float)hi[1])));
+      } else {
         const cs_h2 hi = __builtin_bit_cast(cs_h2, __builtin_amdgcn_cvt_pkrtz(a, b));
         pb.w[k >> 1][ub][0][w] = __builtin_bit_cast(uint32_t, hi);
         pb.w[k >> 1][ub][1][w] =
@@ -417,14 +473,15 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
       }
     }
   };
-  auto stat_at = [&](uint32_t st, int a, int k) __attribute__((always_inline)) {
-    return st + (k >> 1) * 512 + a * 128 + (8 * g + 4 * (k & 1)) * 4;
+  // statistic a of subtile k's streamed rows, sg = a group's statistics plus 32 g
+  auto stat_at = [&](uint32_t sg, int a, int k) __attribute__((always_inline)) {
+    return sg + (k >> 1) * (32 * SROW) + a * 128 + (k & 1) * 16;
   };
   // f(k, ub, r, whether this element is its streamed row's label, x(k)[r])
-  auto each_hit = [&](uint32_t st, auto&& x, auto&& f) __attribute__((always_inline)) {
+  auto each_hit = [&](uint32_t sg, auto&& x, auto&& f) __attribute__((always_inline)) {
 #pragma unroll
     for (int k = 0; k < 2 * SG; ++k) {
-      const u32x4 lb = cs_lds<u32x4>(stat_at(st, CS_LAB, k));
+      const u32x4 lb = cs_lds<u32x4>(stat_at(sg, CS_LAB, k));
       const f32x4 xk = x(k);
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
@@ -437,21 +494,35 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
   // Before a group's exponentials (its first streamed row is n0): the label's term leaves them and the
   // running maximum is raised (up, al: what that multiplies O and l by). Both are rare, and what they
   // change is small, so the common path has no branch between its matrix and vector instructions.
-  auto prepare = [&](int64_t n0, uint32_t st, Scores& s, float (&al)[UB], bool& up, bool& hit) __attribute__((always_inline)) {
+  auto prepare = [&](int64_t n0, int ln, uint32_t st, uint32_t sg, Scores& s, float (&al)[UB], float (&kg)[UB], bool& up, bool& hit)
+      __attribute__((always_inline)) {
     up = hit = false;
+    bool one = true;
+    float e0 = 0.f;
     if constexpr (MODE == CS_COL) {
       if constexpr (NP == 2) {
-        // log2 p = s k_n - lse2_n
+        // log2 p = s k_n f_v - lse2_n (s k_n first: that is finite in a row that takes no part, which has k_n = 1)
+        if (same) {
 #pragma unroll
-        for (int k = 0; k < 2 * SG; ++k) {
-          const f32x4 ls = cs_lds<f32x4>(stat_at(st, CS_LSE2, k)), kn = cs_lds<f32x4>(stat_at(st, CS_KX, k));
+          for (int k = 0; k < 2 * SG; ++k) {
+            const f32x4 ls = cs_lds<f32x4>(stat_at(sg, CS_LSE2, k)), kn = cs_lds<f32x4>(stat_at(sg, CS_KX, k)) * f0;
 #pragma unroll
-          for (int ub = 0; ub < UB; ++ub)
+            for (int ub = 0; ub < UB; ++ub)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) s.v[k][ub][r] = __builtin_fmaf(s.v[k][ub][r], kn[r], -ls[r]);
+              for (int r = 0; r < 4; ++r) s.v[k][ub][r] = __builtin_fmaf(s.v[k][ub][r], kn[r], -ls[r]);
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < 2 * SG; ++k) {
+            const f32x4 ls = cs_lds<f32x4>(stat_at(sg, CS_LSE2, k)), kn = cs_lds<f32x4>(stat_at(sg, CS_KX, k));
+#pragma unroll
+            for (int ub = 0; ub < UB; ++ub)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) s.v[k][ub][r] = __builtin_fmaf(s.v[k][ub][r] * kn[r], kq[ub], -ls[r]);
+          }
         }
       }
-      const int ll = lane & (32 * SG - 1);
+      const int ll = ln & (32 * SG - 1);
       const int32_t lb = cs_lds<int32_t>(st + (ll >> 5) * 512 + CS_LAB * 128 + (ll & 31) * 4) >> 1;
       hit = __any((uint32_t)(lb - (int32_t)r0) < (uint32_t)(16 * UB));
       // the label's element is to become |a| q (its sign follows in `patch`): fp32's scores are log2 p here;
@@ -460,11 +531,11 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
       if (hit) {
         asm volatile("");  // keeps the rare path a branch
         each_hit(
-            st,
+            sg,
             [&](int k) __attribute__((always_inline)) {
-              f32x4 x = cs_lds<f32x4>(stat_at(st, CS_LQ, k));
+              f32x4 x = cs_lds<f32x4>(stat_at(sg, CS_LQ, k));
               if constexpr (NP == 1) {
-                const f32x4 ls = cs_lds<f32x4>(stat_at(st, CS_LSE2, k));
+                const f32x4 ls = cs_lds<f32x4>(stat_at(sg, CS_LSE2, k));
 #pragma unroll
                 for (int r = 0; r < 4; ++r) x[r] = ls[r] == INFINITY ? 0.f : (x[r] + ls[r]) * (1.f / kw);
               }
@@ -475,6 +546,32 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
             });
       }
     } else {
+      if constexpr (NP == 2) {
+        // the items' scales: one for the group, or one each (then in the scores, the group's being 1)
+        const int ll = ln & (32 * SG - 1);
+        const float we = cs_lds<float>(st + (ll >> 5) * 256 + CS_WE * 128 + (ll & 31) * 4);
+        e0 = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, we)));
+        one = e0 < INFINITY && !__any(!(we == e0));
+        if (!one) {
+          asm volatile("");  // keeps the rare path a branch
+          e0 = 0.f;
+#pragma unroll
+          for (int k = 0; k < 2 * SG; ++k) {
+            const f32x4 f = cs_lds<f32x4>(stat_at(sg, CS_WF, k)), w = cs_lds<f32x4>(stat_at(sg, CS_WE, k));
+#pragma unroll
+            for (int ub = 0; ub < UB; ++ub)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                // an item that is not finite: a score of -infinity leaves the sum, any other is NaN
+                const float x = s.v[k][ub][r] * f[r], y = x * w[r];
+                s.v[k][ub][r] = w[r] < INFINITY ? x : y < 0.f ? y : NAN;
+              }
+          }
+        }
+        const float f0 = __builtin_bit_cast(float, (127 - (int)e0) << 23);
+#pragma unroll
+        for (int ub = 0; ub < UB; ++ub) kg[ub] = fminf(fmaxf(kq[ub] * f0, FLT_MIN), FLT_MAX);
+      }
       bool mine = false;
 #pragma unroll
       for (int ub = 0; ub < UB; ++ub) mine |= (uint32_t)(lab[ub] - (int32_t)n0) < 32u * SG;
@@ -505,7 +602,25 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
         for (int k = 0; k < 2 * SG; ++k)
 #pragma unroll
           for (int r = k == 0 ? 2 : 0; r < 4; r += 2) z = fmaxf(fmaxf(s.v[k][ub][r], s.v[k][ub][r + 1]), z);
-        mx[ub] = (MODE == CS_COL ? z : z * kq[ub]) - ps;
+        mx[ub] = MODE == CS_COL ? z : NP == 1 ? z * kq[ub] : __builtin_fmaf(z, kg[ub], -e0);
+      }
+      if constexpr (MODE != CS_COL && NP == 2)  // the maximum is that of exp s times the item's factor
+        if (!one) {
+          asm volatile("");  // keeps the rare path a branch
+#pragma unroll
+          for (int ub = 0; ub < UB; ++ub) mx[ub] = -INFINITY;
+#pragma unroll
+          for (int k = 0; k < 2 * SG; ++k) {
+            const f32x4 w = cs_lds<f32x4>(stat_at(sg, CS_WE, k));
+#pragma unroll
+            for (int ub = 0; ub < UB; ++ub)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) mx[ub] = fmaxf(__builtin_fmaf(s.v[k][ub][r], kg[ub], -w[r]), mx[ub]);
+          }
+        }
+#pragma unroll
+      for (int ub = 0; ub < UB; ++ub) {
+        mx[ub] -= ps;
         mine |= mx[ub] > m[ub];
       }
       up = __any(mine);
@@ -516,25 +631,25 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
           x = fmaxf(x, __shfl_xor(x, 32, 64));
           x = fmaxf(x, m[ub]);
           al[ub] = __builtin_amdgcn_exp2f(m[ub] - x);
+          l[ub] *= cs_exp2_d<NP>(m[ub] - x);
           m[ub] = x;
-          l[ub] *= (double)al[ub];
         }
       }
     }
   };
   // the label's element of P is negative
-  auto patch = [&](uint32_t st, Probs& pb) __attribute__((always_inline)) {
-    each_hit(st, [](int) { return f32x4{}; }, [&](int k, int ub, int r, bool is, float) __attribute__((always_inline)) {
+  auto patch = [&](uint32_t sg, Probs& pb) __attribute__((always_inline)) {
+    each_hit(sg, [](int) { return f32x4{}; }, [&](int k, int ub, int r, bool is, float) __attribute__((always_inline)) {
       const uint32_t sign = is ? (r & 1 ? 0x80000000u : 0x8000u) : 0u;
 #pragma unroll
       for (int pl = 0; pl < NP; ++pl) pb.w[k >> 1][ub][pl][2 * (k & 1) + (r >> 1)] ^= sign;
     });
   };
   // rows of negative weight
-  auto negate = [&](uint32_t st, Probs& pb) __attribute__((always_inline)) {
+  auto negate = [&](uint32_t sg, Probs& pb) __attribute__((always_inline)) {
 #pragma unroll
     for (int k = 0; k < 2 * SG; ++k) {
-      const u32x4 lb = cs_lds<u32x4>(stat_at(st, CS_LAB, k));
+      const u32x4 lb = cs_lds<u32x4>(stat_at(sg, CS_LAB, k));
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -545,19 +660,21 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
     }
   };
   // exponentials of part i = (subtile k, ub) of 2 SG UB
-  auto exponentials = [&](int i, uint32_t st, const Scores& s, Probs& pb, float (&sum)[UB]) __attribute__((always_inline)) {
+  auto exponentials = [&](int i, uint32_t sg, const Scores& s, Probs& pb, const float (&kg)[UB], float (&sum)[UB])
+      __attribute__((always_inline)) {
     const int k = i / UB, ub = i % UB;
-    f32x4 ls, e;
-    if constexpr (MODE == CS_COL && NP == 1) ls = cs_lds<f32x4>(stat_at(st, CS_LSE2, k));
+    f32x4 ls, e, f = {};
+    if constexpr (MODE == CS_COL && NP == 1) ls = cs_lds<f32x4>(stat_at(sg, CS_LSE2, k));
+    if constexpr (MODE == CS_ROW && NP == 2) f = cs_lds<f32x4>(stat_at(sg, CS_WF, k));
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const float x = s.v[k][ub][r];
-      if constexpr (MODE != CS_COL) e[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x, kq[ub], -m[ub]));
+      if constexpr (MODE != CS_COL) e[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x, NP == 2 ? kg[ub] : kq[ub], -m[ub]));
       else if constexpr (NP == 2) e[r] = __builtin_amdgcn_exp2f(x - m[ub]);
       else e[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x, kw, -ls[r]));
     }
     if constexpr (MODE != CS_COL) sum[ub] += (e[0] + e[1]) + (e[2] + e[3]);
-    if constexpr (MODE != CS_STATS) pack(pb, k, ub, e);
+    if constexpr (MODE != CS_STATS) pack(pb, k, ub, e, f);
   };
   // O and l follow a raised maximum (bf16; with fp32 operands the product does it for O)
   auto rescale = [&](bool up, const float (&al)[UB]) __attribute__((always_inline)) {
@@ -574,7 +691,7 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
   int buf = 0;
   for (int64_t t = tb0; t < tb1; ++t) {
     if (t + AHEAD > tb1) cs_wait<0>();
-    else if (MODE == CS_COL && wave == 0) cs_wait<(AHEAD - 1) * (CPT * NP + 1)>();
+    else if (SROW > 0 && wave == 0) cs_wait<(AHEAD - 1) * (CPT * NP + 1)>();
     else cs_wait<(AHEAD - 1) * CPT * NP>();
     __syncthreads();
     if (t + AHEAD < tb1) copy(t + AHEAD, buf == 0 ? NB - 1 : buf - 1);
@@ -582,27 +699,33 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
 #pragma unroll
       for (int gr = 0; gr < GROUPS; ++gr) {
         const int64_t n0 = t * KT + 32 * SG * gr;
-        const uint32_t bo = buf * BUF + 32 * SG * gr * ROWB, st = lds0 + buf * BUF + IMG + 512 * SG * gr;
-        float al[UB], sum[UB] = {};
+        const uint32_t bo = buf * BUF + 32 * SG * gr * ROWB, st = lds0 + buf * BUF + IMG + 32 * SG * gr * SROW;
+        int ln = lane;
+        // fp32 has no registers to spare: what follows from the lane is formed here again, not held in registers (a
+        // reload from scratch would also wait for the copies in flight), the statistics' offsets stay in the instructions
+        if constexpr (NP == 2) asm volatile("" : "+v"(ln));
+        uint32_t sg = st + 32 * (ln >> 4);
+        if constexpr (NP == 2) asm("" : "+v"(sg));
+        float al[UB], kg[UB], sum[UB] = {};
         bool up, hit;
         Scores s;
         Probs pb;
-        scores(bo, s);
-        prepare(n0, st, s, al, up, hit);
+        scores(ln, bo, s);
+        prepare(n0, ln, st, sg, s, al, kg, up, hit);
         rescale(up, al);
 #pragma unroll
-        for (int i = 0; i < 2 * SG * UB; ++i) exponentials(i, st, s, pb, sum);
+        for (int i = 0; i < 2 * SG * UB; ++i) exponentials(i, sg, s, pb, kg, sum);
         if constexpr (MODE != CS_COL)
 #pragma unroll
           for (int ub = 0; ub < UB; ++ub) l[ub] += (double)sum[ub];
         if constexpr (MODE == CS_COL) {
           if (hit) {
             asm volatile("");  // keeps the rare path a branch
-            patch(st, pb);
+            patch(sg, pb);
           }
-          if (flip) negate(st, pb);
+          if (flip) negate(sg, pb);
         }
-        if constexpr (MODE != CS_STATS) product(bo, pb, al);
+        if constexpr (MODE != CS_STATS) product(ln, bo, pb, al);
       }
     buf = buf + 1 == NB ? 0 : buf + 1;
   }
@@ -610,8 +733,13 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
 #pragma unroll
   for (int ub = 0; ub < UB; ++ub) {
     const int64_t q = r0 + 16 * ub + i16;
-    float sum = (float)l[ub];
-    if constexpr (MODE != CS_COL) {
+    double sum = l[ub];
+    if constexpr (MODE != CS_COL && NP == 1) {
+      float f = (float)sum;
+      f += __shfl_xor(f, 16, 64);
+      f += __shfl_xor(f, 32, 64);
+      sum = f;
+    } else if constexpr (MODE != CS_COL) {  // may pass fp32's range
       sum += __shfl_xor(sum, 16, 64);
       sum += __shfl_xor(sum, 32, 64);
     }
@@ -671,7 +799,8 @@ struct CsFew {
   int64_t steps;  // of 64 items, dealt to the workgroups in turn
   float kbase;
   int32_t* lab;
-  float *m, *l;
+  float* m;
+  double* l;
   unsigned int* done;
 };
 template <int DP, int Q>
@@ -772,29 +901,6 @@ __device__ __forceinline__ float cs_finite_abs(float x) {
   const float a = fabsf(x);
   return a <= FLT_MAX ? a : 0.f;
 }
-__device__ __forceinline__ float cs_block_max(float v, float* sh) {
-  v = wave_max(v);
-  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
-  __syncthreads();
-  v = sh[0];
-  for (unsigned i = 1; i < blockDim.x / 64; ++i) v = fmaxf(v, sh[i]);
-  return v;
-}
-
-// largest finite |w| of each workgroup's share
-__global__ __launch_bounds__(256) void cs_amax_kernel(const float* __restrict__ w, int64_t n, float* __restrict__ part) {
-  __shared__ float sh[4];
-  float a = 0.f;
-  const int64_t n4 = n / 4, step = (int64_t)gridDim.x * 256;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n4; i += step) {
-    const f32x4 v = *reinterpret_cast<const f32x4*>(w + 4 * i);
-    a = fmaxf(fmaxf(fmaxf(cs_finite_abs(v[0]), cs_finite_abs(v[1])), fmaxf(cs_finite_abs(v[2]), cs_finite_abs(v[3]))), a);
-  }
-  if (blockIdx.x == 0 && threadIdx.x < n - 4 * n4) a = fmaxf(a, cs_finite_abs(w[4 * n4 + threadIdx.x]));
-  a = cs_block_max(a, sh);
-  if (threadIdx.x == 0) part[blockIdx.x] = a;
-}
-
 // the power of two that brings a into [2^13, 2^14)
 __device__ __forceinline__ int cs_exp(float a) {
   if (!(a > 0.f)) return 0;
@@ -807,42 +913,32 @@ __device__ __forceinline__ int cs_exp(float a) {
 struct CsImage {
   const void *x, *w;
   char *ximg, *wimg;       // wimg null: w is read as it is
-  int64_t N, Npad, V, D;
+  int64_t N, Npad, V, Vpad, D;
   int64_t xplane, wplane;
   int64_t ignore;
   const int64_t* labels;
   int32_t* lab;
-  float* kx;
-  const float* part;
+  float *kx, *wstat;
   CsScal* scal;
   unsigned int* done;
   int xblocks;
 };
 
-// x [N, D] and w [V, D] into padded 16-bit rows: two fp16 planes of the scaled values (fp32), a copy
-// (bf16). A row of x whose label is the ignored one keeps its finite entries only (its weight in the
+// x [N, D] and w [V, D] into padded 16-bit rows: two fp16 planes of the scaled values (fp32), with w's
+// statistics (up to a whole tile), or a copy (bf16). A row of x whose label is the ignored one keeps its finite entries only (its weight in the
 // column pass is zero, and zero times infinity would not be). 4 columns per lane.
 template <int DP, int NP>
 __global__ __launch_bounds__(256) void cs_image_kernel(CsImage p) {
   constexpr int LPR = DP / 4, RPB = 256 / LPR;  // lanes per row, rows per workgroup
-  __shared__ float sh[4];
   const int c = (threadIdx.x % LPR) * 4, rr = threadIdx.x / LPR;
   const bool is_x = (int)blockIdx.x < p.xblocks;
-  float wscale = 1.f;
-  if (NP == 2 && !is_x) {
-    float a = 0.f;
-    for (int i = threadIdx.x; i < CS_AMAX_BLOCKS; i += 256) a = fmaxf(a, p.part[i]);
-    const int e = cs_exp(cs_block_max(a, sh));
-    wscale = ldexpf(1.f, e);
-    if ((int)blockIdx.x == p.xblocks && threadIdx.x == 0) p.scal->w_inv = ldexpf(1.f, -e);
-  }
   if (blockIdx.x == 0) {
     if (threadIdx.x < 4) p.scal->zero[threadIdx.x] = 0.f;
     ticket_zero(p.done, threadIdx.x, 256);
   }
   const int64_t blk = is_x ? blockIdx.x : blockIdx.x - p.xblocks;
   const int64_t nblk = is_x ? p.xblocks : gridDim.x - p.xblocks;
-  const int64_t rows = is_x ? p.N : p.V, rows_pad = is_x ? p.Npad : p.V;
+  const int64_t rows = is_x ? p.N : p.V, rows_pad = is_x ? p.Npad : NP == 2 ? p.Vpad : p.V;
   const void* src = is_x ? p.x : p.w;
   char* dst = is_x ? p.ximg : p.wimg;
   const int64_t plane = is_x ? p.xplane : p.wplane;
@@ -886,17 +982,34 @@ __global__ __launch_bounds__(256) void cs_image_kernel(CsImage p) {
             if (c + j < p.D) v[j] = s[j];
         }
       }
-      float sc = wscale;
-      if (is_x) {
-        if (lb < 0)
-          for (int j = 0; j < 4; ++j) v[j] = fabsf(v[j]) <= FLT_MAX ? v[j] : 0.f;
-        float a = fmaxf(fmaxf(cs_finite_abs(v[0]), cs_finite_abs(v[1])), fmaxf(cs_finite_abs(v[2]), cs_finite_abs(v[3])));
+      if (is_x && lb < 0)
+        for (int j = 0; j < 4; ++j) v[j] = fabsf(v[j]) <= FLT_MAX ? v[j] : 0.f;
+      float a = fmaxf(fmaxf(cs_finite_abs(v[0]), cs_finite_abs(v[1])), fmaxf(cs_finite_abs(v[2]), cs_finite_abs(v[3])));
 #pragma unroll
-        for (int o = LPR / 2; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor(a, o, 64));
-        const int e = cs_exp(a);
-        sc = ldexpf(1.f, e);
+      for (int o = LPR / 2; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor(a, o, 64));
+      int e = cs_exp(a);
+      if (is_x) {
         if (c == 0) p.kx[r] = ldexpf(1.f, -e);
+      } else {
+        e = !(a > 0.f) || e > CS_WE_MAX ? CS_WE_MAX : ((e - 3) & ~7) + 3;
+        int odd = 0;  // 1: an infinite entry, 2: a NaN
+        for (int j = 0; j < 4; ++j) odd = isnan(v[j]) ? 2 : isinf(v[j]) && odd < 1 ? 1 : odd;
+#pragma unroll
+        for (int o = LPR / 2; o > 0; o >>= 1) {
+          const int b = __shfl_xor(odd, o, 64);
+          odd = odd > b ? odd : b;
+        }
+        if (odd) {
+          e = 0;
+          for (int j = 0; j < 4; ++j) v[j] = isinf(v[j]) ? copysignf(0x1p14f, v[j]) : 0.f;
+        }
+        if (c == 0) {
+          p.wstat[cs_wstat(r, CS_WF)] = odd ? 0x1p90f : ldexpf(1.f, -e - 1);
+          p.wstat[cs_wstat(r, CS_WE)] = odd == 2 ? NAN : odd ? INFINITY : (float)(e + 1);
+        }
+        if (r >= rows) continue;  // past the last item: statistics alone
       }
+      const float sc = ldexpf(1.f, e);
       uint32_t h[2], lo[2];
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
@@ -918,7 +1031,8 @@ struct CsRows {
   int bf16;
   int64_t N, Npad, V, D;
   int nsplit;
-  const float *m, *l, *O;
+  const float *m, *O;
+  const double* l;
   const int32_t* lab;
   const float* weights;
   const float* kx;
@@ -996,11 +1110,10 @@ __device__ __forceinline__ void cs_row(const CsRows& p) {
   const int64_t n = NWV == 1 ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x;
   const bool first = NWV == 1 || wave == 0;
   if (n >= p.Npad) return;
-  const float kw = NP == 2 ? p.kbase * p.scal->w_inv : p.kbase;
   if (n >= p.N) {
     if (first && lane == 0 && p.stat) {
       p.stat[cs_stat(n, CS_LSE2)] = INFINITY;
-      p.stat[cs_stat(n, CS_KX)] = kw;
+      p.stat[cs_stat(n, CS_KX)] = 1.f;
       reinterpret_cast<int32_t*>(p.stat)[cs_stat(n, CS_LAB)] = -1;
       p.stat[cs_stat(n, CS_LQ)] = 0.f;
     }
@@ -1043,7 +1156,7 @@ __device__ __forceinline__ void cs_row(const CsRows& p) {
   double L = 0.;
 #pragma unroll 4
   for (int s = lane; s < p.nsplit; s += 64)
-    L += (double)p.l[n * p.nsplit + s] * (double)__builtin_amdgcn_exp2f(ms[s] - M);
+    L += p.l[n * p.nsplit + s] * cs_exp2_d<NP>(ms[s] - M);
   L = wave_sum_d(L);
   // in log2 units: the other items' log sum and the label's logit. Logarithms of fp32 mantissas (error
   // below 2^-23), sums with the exponents in 64 bits: the 64-bit logarithm, on every row, took most of
@@ -1072,7 +1185,8 @@ __device__ __forceinline__ void cs_row(const CsRows& p) {
     if (NP == 2) ca += ilogbf(p.kx[n]) + CS_XREF;
     // NaN statistics of a labelled row reach every item's gradient, as the formula's do
     p.stat[cs_stat(n, CS_LSE2)] = live ? (float)(lse2 - ca) : INFINITY;
-    p.stat[cs_stat(n, CS_KX)] = NP == 2 ? fminf(fmaxf(kw * p.kx[n], FLT_MIN), FLT_MAX) : kw;
+    // (a row that takes no part: a factor whose product with any score is finite)
+    p.stat[cs_stat(n, CS_KX)] = NP == 2 && live ? fminf(fmaxf(2.f * p.kbase * p.kx[n], FLT_MIN), FLT_MAX) : 1.f;
     reinterpret_cast<int32_t*>(p.stat)[cs_stat(n, CS_LAB)] = live ? 2 * lb + (a < 0.f) : lb;
     p.stat[cs_stat(n, CS_LQ)] = (float)(o2 - lse2 + ca);
   }
@@ -1080,12 +1194,12 @@ __device__ __forceinline__ void cs_row(const CsRows& p) {
   // statistic takes a finite score out, not an infinite one; fp32's scores are of scaled values)
   if (NP == 1 && p.stat && lb < 0 && lane < LPR) *reinterpret_cast<u32x2*>(p.ximg + n * (2 * DP) + 2 * c) = u32x2{0, 0};
   if (!p.dx || lane >= LPR) return;
-  const float il = L == 0. ? 0.f : (float)((NP == 2 ? (double)p.scal->w_inv : 1.) / L);
+  const double il = L == 0. ? 0. : (NP == 2 ? 2. : 1.) / L;  // fp32: O holds half its items (f = 2^(-e - 1)); L may pass fp32's range
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     if (c + j >= p.D) continue;
     float v = 0.f;
-    if (lb >= 0) v = L == 0. ? 0.f : a * q * (o[j] * il - wv[j]);
+    if (lb >= 0) v = L == 0. ? 0.f : a * q * (NP == 2 ? (float)(o[j] * il) - wv[j] : o[j] * (float)il - wv[j]);
     else if (lb == -2) v = NAN;
     p.dx[n * p.D + c + j] = v;
   }
@@ -1183,7 +1297,7 @@ CsSpread cs_spread(int64_t nrb, int64_t tiles, const CsCfg& c, int D, int NP, in
 }
 
 struct CsShape {
-  int64_t N, Npad, V, D;
+  int64_t N, Npad, V, Vpad, D;
   int DP, NP, es;
   bool wimage, few;
   int rsplit;
@@ -1200,6 +1314,7 @@ CsShape cs_plan(int64_t N, int64_t V, int64_t D, int dtype, int want) {
   s.NP = dtype == RS_DTYPE_F32 ? 2 : 1;
   s.es = dtype == RS_DTYPE_F32 ? 4 : 2;
   s.Npad = (N + 63) / 64 * 64;
+  s.Vpad = (V + 63) / 64 * 64;
   s.wimage = s.NP == 2 || D % 8 != 0;
   const CsCfg rc = cs_cfg(s.DP, s.NP, want & RS_CATALOG_DX ? CS_ROW : CS_STATS), cc = cs_cfg(s.DP, s.NP, CS_COL);
   s.rtiles = ceil_div(V, rc.KT);
@@ -1240,7 +1355,7 @@ struct CsKeep {
   CsScal* scal;
   char *ximg, *wimg;
   int32_t* lab;
-  float *kx, *stat, *dx;
+  float *kx, *wstat, *stat, *dx;
   bool ok;
   size_t bytes;
   CsKeep(void* base, size_t size, const CsShape& s, int want) {
@@ -1250,6 +1365,7 @@ struct CsKeep {
     wimg = s.wimage ? c.take<char>((size_t)s.V * s.DP * 2 * s.NP) : nullptr;
     lab = c.take<int32_t>(s.Npad);
     kx = c.take<float>(s.Npad);
+    wstat = s.wimage && s.NP == 2 ? c.take<float>(s.Vpad * 2) : nullptr;
     stat = c.take<float>(s.Npad * 4);
     dx = want & RS_CATALOG_DX ? c.take<float>((size_t)s.N * s.D) : nullptr;
     bytes = align_up(c.off, 256);
@@ -1258,15 +1374,15 @@ struct CsKeep {
 };
 struct CsFwdWs {
   unsigned int* done;
-  float *part, *m, *l, *O;
+  float *m, *O;
+  double* l;
   bool ok;
   size_t bytes;
   CsFwdWs(void* base, size_t size, const CsShape& s, int want) {
     Carve c(base, size);
     done = c.take<unsigned int>(TICKET_WORDS);
-    part = c.take<float>(CS_AMAX_BLOCKS);
     m = c.take<float>((size_t)s.rsplit * s.N);
-    l = c.take<float>((size_t)s.rsplit * s.N);
+    l = c.take<double>((size_t)s.rsplit * s.N);
     O = want & RS_CATALOG_DX ? c.take<float>((size_t)s.rsplit * s.N * s.DP) : nullptr;
     bytes = align_up(c.off, 256);
     ok = c.ok();
@@ -1358,11 +1474,10 @@ extern "C" int rs_catalog_softmax_fwd(const void* X, const void* W, const int64_
     CS_GO(256, 1) CS_GO(256, 2)
 #undef CS_GO
   } else if (N > 0) {
-    if (s.NP == 2) hipLaunchKernelGGL(cs_amax_kernel, dim3(CS_AMAX_BLOCKS), dim3(256), 0, st, (const float*)W, V * D, w.part);
     const int rpb = 256 / (s.DP / 4);
-    CsImage im{X,    W,    k.ximg, k.wimg, N, s.Npad, V, D, s.Npad * s.DP * 2, V * s.DP * 2, ignore_index, labels, k.lab,
-               k.kx, w.part, k.scal, w.done, 0};
-    int64_t xb = ceil_div(s.Npad, rpb), wb = s.wimage ? ceil_div(V, rpb) : 0;
+    CsImage im{X, W, k.ximg, k.wimg, N, s.Npad, V, s.Vpad, D, s.Npad * s.DP * 2, V * s.DP * 2, ignore_index, labels, k.lab,
+               k.kx, k.wstat, k.scal, w.done, 0};
+    int64_t xb = ceil_div(s.Npad, rpb), wb = s.wimage ? ceil_div(s.NP == 2 ? s.Vpad : V, rpb) : 0;
     im.xblocks = (int)(xb < 2048 ? xb : 2048);
     if (wb > 4096) wb = 4096;
     const dim3 gi((unsigned)(im.xblocks + wb));
@@ -1391,7 +1506,8 @@ extern "C" int rs_catalog_softmax_fwd(const void* X, const void* W, const int64_
     p.scal = k.scal;
     p.scale = scale;
     p.kbase = kbase;
-    p.kx = k.kx;
+    p.kr = k.kx;
+    p.stat = k.wstat;
     p.lab = k.lab;
     p.m = w.m;
     p.l = w.l;
@@ -1399,7 +1515,7 @@ extern "C" int rs_catalog_softmax_fwd(const void* X, const void* W, const int64_
     if (want & RS_CATALOG_DX) cs_launch_pass<CS_ROW>(s, p, s.rnrb * s.rsplit, st);
     else cs_launch_pass<CS_STATS>(s, p, s.rnrb * s.rsplit, st);
   }
-  const CsRows r{X, W, s.NP == 1, N, s.Npad, V, D, s.rsplit, w.m, w.l, w.O, k.lab, weights, k.kx, scale, kbase, row_loss,
+  const CsRows r{X, W, s.NP == 1, N, s.Npad, V, D, s.rsplit, w.m, w.O, w.l, k.lab, weights, k.kx, scale, kbase, row_loss,
                  lse, k.dx, want & RS_CATALOG_DW ? k.stat : nullptr, k.ximg, k.scal,
                  N <= CS_TAIL_ROWS ? w.done : nullptr, mean, loss};
   if (N > 0) {
@@ -1463,6 +1579,7 @@ extern "C" int rs_catalog_softmax_bwd(const void* W, int64_t N, int64_t V, int64
     p.scal = k.scal;
     p.scale = scale;
     p.kbase = (float)((double)scale * CS_LOG2E);
+    p.kr = k.wstat;
     p.stat = k.stat;
     p.m = w.m;
     p.O = w.O;

@@ -31,18 +31,19 @@ def test_excluded_rows_may_hold_the_largest_values(cuda, dtype, N, D):
 
 def masked(N, V, D, dtype, bias, seed=0):
     """x's last column is 1, w's the item's bias; every seventh item is masked by it. Ignored rows are
-    zeros, as a padded batch has them. Labels are items that are not masked."""
+    zeros, as a padded batch has them, or favour the masked items. Labels are items that are not masked."""
     x, w, y, _ = inputs(N, V, D, dtype, seed=seed, ignored=0.2)
     x[:, -1] = 1.0
-    x[y == IGN] = 0.0
+    x[y == IGN, -1] = -1.0
+    x[(y == IGN) & (torch.arange(N, device="cuda") % 2 == 0)] = 0.0
     gone = torch.arange(V, device="cuda") % 7 == 3
     w[:, -1] = torch.where(gone, torch.full_like(w[:, -1], bias), 0.25 * w[:, -1])
     y = torch.where(y == IGN, y, torch.where(gone[y.clamp(min=0)], y.clamp(min=0) + 1, y) % V)
     return x, w, y, gone
 
 
-@pytest.mark.parametrize("dtype", [torch.bfloat16], ids=["bf16"])
-@pytest.mark.parametrize("bias", [-1e4, -1e9, -1e30, -float("inf")])
+@DTYPES
+@pytest.mark.parametrize("bias", [-1e4, -1e9, -1e30, -3.3e38, -float("inf")])
 @pytest.mark.parametrize("N,V,D", [(40, 500, 64), (64, 701, 96), (65, 701, 100), (130, 1000, 128), (300, 259, 256)])
 def test_masked_items(cuda, dtype, bias, N, V, D):
     """A masked item changes no other item's logit: loss and gradients are those of the catalogue without it,
@@ -59,9 +60,66 @@ def test_masked_items(cuda, dtype, bias, N, V, D):
     within(row2, r["row"], t["row"], "row (loss alone)")
     within(loss, r["loss"], t["loss"], "loss")
     within(l2, r["loss"], t["loss"], "loss alone")
-    live = (y != IGN).cpu()
+    live = (y != IGN).cpu()   # (the others' lse is infinite where they favour a masked item)
     within(lse.cpu()[live], r["lse"][live], t["row"][live], "lse")
     within(dw[~gone], r["dw"], t["dw"], "dw")
     assert not bool(dw[gone].any())
     cols = D - 1 if bias == -float("inf") else D
     within(dx[:, :cols], r["dx"][:, :cols], t["dx"][:, :cols], "dx")
+
+
+@DTYPES
+@pytest.mark.parametrize("N,V,D", [(40, 500, 64), (130, 1000, 128), (300, 600, 256), (70, 5000, 100)])
+def test_items_of_different_scales(cuda, dtype, N, V, D):
+    """Items from 1e-9 to 1 in size, the larger ones unlikely (a bias of -12): small and large items weigh alike
+    in dX, and each item's probability is its own."""
+    x, w, y, _ = inputs(N, V, D, dtype, seed=N, spread=1.5)
+    x[:, -1] = 1.0
+    size = torch.logspace(-9, 0, V, device="cuda")[torch.randperm(V, generator=torch.Generator().manual_seed(2)).cuda()]
+    w = (w.float() * size[:, None]).to(dtype)
+    w[:, -1] = torch.where(size > 1e-6, torch.full_like(w[:, -1], -12.0), torch.zeros_like(w[:, -1]))
+    w[5] = 0.0
+    r = reference(x, w, y)
+    t = tolerances(r, N, V, D, dtype)
+    loss, row, dx, dw = step(x, w, y)
+    within(row, r["row"], t["row"], "row")
+    within(loss, r["loss"], t["loss"], "loss")
+    within(dx, r["dx"], t["dx"], "dx")
+    within(dw, r["dw"], t["dw"], "dw")
+
+
+@pytest.mark.parametrize("sx,sw", [(1e30, 1e-30), (1e-28, 1e28), (1.0, 1e-25)])
+def test_far_scales_of_all_items(cuda, sx, sw):
+    """The whole catalogue far from one, a zero item in it, with rows that make up for it."""
+    x, w, y, _ = inputs(90, 400, 96, torch.float32, seed=5)
+    x, w = x * sx, w * sw
+    w[7] = 0.0
+    r = reference(x, w, y)
+    t = tolerances(r, 90, 400, 96, torch.float32)
+    loss, row, dx, dw = step(x, w, y)
+    within(row, r["row"], t["row"], "row")
+    within(dx, r["dx"], t["dx"] + 2.0 ** -126, "dx")
+    within(dw, r["dw"], t["dw"] + 2.0 ** -126, "dw")
+
+
+def test_infinite_and_nan_items(cuda):
+    """float32: an item's single infinite entry gives its logit the sign that the row's entry gives it, zero times
+    infinity and a NaN entry every row NaN, as the products do; with and without gradients."""
+    F = pkg("functional")
+    for N in (40, 130):
+        x, w, y, _ = inputs(N, 300, 64, torch.float32, seed=N)
+        y = torch.where(y == 9, y + 1, y)
+        x[:, 3] = x[:, 3].abs() + 0.5
+        x[3, 3], x[4, 3] = -0.5, 0.0
+        w2 = w.clone()
+        w2[9, 3] = -float("inf")
+        ref = reference(x, torch.cat([w[:9], w[10:]]), torch.where(y > 9, y - 1, y))
+        t = tolerances(ref, N, 300, 64, torch.float32)
+        keep = torch.ones(N, dtype=torch.bool)
+        keep[3:5] = False
+        for row in (step(x, w2, y)[1], F.catalog_softmax_fwd(x, w2, y, want_grad=False)[1]):
+            within(row.cpu()[keep], ref["row"][keep], t["row"][keep], "row")
+            assert not bool(row[3:5].isfinite().any()) and bool(row[4].isnan())
+        w2[9, 3] = float("nan")
+        loss, row, dx, dw = step(x, w2, y)
+        assert bool(row.isnan().all()) and bool(dx.isnan().all()) and bool(dw.isnan().all())
