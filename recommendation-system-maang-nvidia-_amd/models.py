@@ -567,9 +567,7 @@ class MultiTaskModel(nn.Module):
         return [p for p in self.parameters() if id(p) not in emb]
 
     def get_config(self):
-        return {"config": self.config.to_dict(), "user_vocab": self.encoder.user_vocab,
-                "item_vocab": self.encoder.item_vocab, "feature_specs": self.encoder.feature_specs,
-                "class_weights": self.class_weights}
+        return {**self.encoder.get_config(), "class_weights": self.class_weights}
 
     @classmethod
     def from_config(cls, config, **kw):

@@ -125,3 +125,16 @@ def test_modules():
     wet = models.MultiTowerModel(cfg, ["a"], ["b"], {}, device="cpu", tower_dropout=0.25)
     again = models.MultiTowerModel.from_config(wet.get_config(), device="cpu")
     assert again.tower_dropout == 0.25 and len(again.item_tower.dropouts) == 1
+
+
+def test_multi_task_config_keeps_the_tower_dropout():
+    """A model rebuilt from its configuration drops alike and takes the original's state; without dropout the
+    configuration holds what it held."""
+    models, cfgm = pkg("models"), pkg("config")
+    cfg = cfgm.ModelConfig(embedding_dim=16, user_tower_dims=[8], item_tower_dims=[8], dnn_dims=[8])
+    wet = models.MultiTaskModel(cfg, ["a"], ["b"], {}, class_weights={0: 0.5, 1: 2.0}, device="cpu", tower_dropout=0.25)
+    again = models.MultiTaskModel.from_config(wet.get_config(), device="cpu")
+    assert again.encoder.tower_dropout == 0.25 and again.class_weights == {0: 0.5, 1: 2.0}
+    again.load_state_dict(wet.state_dict())
+    plain = models.MultiTaskModel(cfg, ["a"], ["b"], {}, device="cpu")
+    assert set(plain.get_config()) == {"config", "user_vocab", "item_vocab", "feature_specs", "class_weights"}
