@@ -24,7 +24,7 @@ import torch
 
 from . import functional as F
 from .config import load_config
-from .models import MultiTowerModel
+from .models import MultiTowerModel, served_state
 
 logger = logging.getLogger(__name__)
 
@@ -67,7 +67,7 @@ class RecommendationService:
         if not enc_state:
             raise ValueError(f"{model_path} holds no encoder weights")
         enc = MultiTowerModel(cfg, self.user_vocab, self.item_vocab, {}, device=self.device)
-        enc.load_state_dict(enc_state)
+        enc.load_state_dict(served_state(enc_state))
         self.model = enc
         self._precompute_item_embeddings()
         logger.info(" Model service ready")

@@ -16,6 +16,7 @@ kernel (optim.py).
 from __future__ import annotations
 
 import math
+import re
 from typing import Any, Dict, List, Optional
 
 import numpy as np
@@ -128,6 +129,12 @@ def set_dropout_seed(module: nn.Module, seed: int) -> None:
     give each rank another seed, or their masks are the same)."""
     for j, m in enumerate(m for m in module.modules() if isinstance(m, Dropout)):
         m.state.copy_(torch.tensor([int(seed) + 7919 * j, 0], dtype=torch.int64))
+
+
+def served_state(state: Dict[str, torch.Tensor]) -> Dict[str, torch.Tensor]:
+    """A model's state without its dropout generators: what a model that only answers takes (it is built
+    without dropout)."""
+    return {k: v for k, v in state.items() if not re.search(r"(^|\.)dropouts\.\d+\.state$", k)}
 
 
 class Tower(nn.Module):

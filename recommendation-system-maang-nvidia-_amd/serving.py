@@ -20,7 +20,7 @@ import torch
 from . import functional as F
 from .config import load_config
 from .faiss_io import read_index_flat
-from .models import MultiTowerModel
+from .models import MultiTowerModel, served_state
 from .retrieval import BruteForceIndex, l2_normalize
 
 logger = logging.getLogger(__name__)
@@ -52,7 +52,7 @@ class RecommendationService:
         cfg = load_config(self.model_dir)          # config.json (+ config_ext.json)
         enc = MultiTowerModel(cfg, self.user_vocab, item_vocab, {}, device=self.device)
         state = torch.load(self.model_dir / "encoder.pt", map_location="cpu", weights_only=True)
-        enc.load_state_dict(state)
+        enc.load_state_dict(served_state(state))
         self.encoder_model = enc
         if (self.model_dir / "faiss.idx").exists():      # app/recommendation_service.py:47
             _, xb = read_index_flat(self.model_dir / "faiss.idx")

@@ -42,7 +42,7 @@ from .config import ModelConfig, save_config
 from .data import make_dataset
 from .faiss_io import write_index_flat
 from .lookup import build_vocab
-from .models import MultiTaskModel
+from .models import MultiTaskModel, served_state
 from .optim import Adagrad, ExponentialDecay
 from .retrieval import BruteForceIndex, ShardedBruteForceIndex, recall_at_k, shard_rows
 
@@ -367,7 +367,8 @@ class ProductionTrainer:
     def _save_artifacts(self, model, datasets):
         """src/trainer.py:228-234: encoder weights, vocabs.json, config.json (reference fields
         only; the build-only fields go to config_ext.json)."""
-        torch.save({k: v.cpu() for k, v in model.encoder.state_dict().items()}, self.output_dir / "encoder.pt")
+        torch.save({k: v.cpu() for k, v in served_state(model.encoder.state_dict()).items()},
+                   self.output_dir / "encoder.pt")
         with open(self.output_dir / "vocabs.json", "w") as f:
             json.dump({"users": datasets["user_vocab"], "items": datasets["item_vocab"]}, f)
         save_config(self.config, self.output_dir)   # config.json keeps the reference schema

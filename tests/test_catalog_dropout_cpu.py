@@ -138,3 +138,33 @@ def test_multi_task_config_keeps_the_tower_dropout():
     again.load_state_dict(wet.state_dict())
     plain = models.MultiTaskModel(cfg, ["a"], ["b"], {}, device="cpu")
     assert set(plain.get_config()) == {"config", "user_vocab", "item_vocab", "feature_specs", "class_weights"}
+
+
+def test_a_model_with_dropout_is_served(tmp_path, monkeypatch):
+    """The artefacts of a model with tower dropout, as the trainer writes them and as its checkpoint holds them, load
+    into the services, whose models have none."""
+    models, cfgm, trainer = pkg("models"), pkg("config"), pkg("trainer")
+    cfg = cfgm.ModelConfig(embedding_dim=16, user_tower_dims=[8], item_tower_dims=[8], dnn_dims=[8])
+    users, items = ["a", "b"], ["c", "d", "e"]
+    wet = models.MultiTaskModel(cfg, users, items, {}, device="cpu", tower_dropout=0.25)
+    tr = trainer.ProductionTrainer.__new__(trainer.ProductionTrainer)
+    tr.config, tr.output_dir = cfg, tmp_path
+    tr._save_artifacts(wet, {"user_vocab": users, "item_vocab": items})
+    torch.save(wet.state_dict(), tmp_path / "best_model.pt")
+    (tmp_path / "item_map.json").write_text('{"0": "c", "1": "d", "2": "e"}')
+    torch.save(torch.eye(3, 16), tmp_path / "item_index.pt")
+    cpu = torch.device("cpu")
+    svc = pkg("serving").RecommendationService(str(tmp_path), cpu)
+    svc.load()
+    ms = pkg("model_service").RecommendationService(str(tmp_path), cpu)
+    monkeypatch.setattr(ms, "_precompute_item_embeddings", lambda: None)   # (GPU kernels)
+    ms.load_model()
+    for enc in (svc.encoder_model, ms.model):
+        want = wet.encoder.state_dict()
+        for k, v in enc.state_dict().items():
+            assert torch.equal(v, want[k]), k
+    # an encoder.pt that holds the generators too
+    torch.save(wet.encoder.state_dict(), tmp_path / "encoder.pt")
+    svc.load()
+    # the generators stay in the model's own state
+    assert "encoder.user_tower.dropouts.0.state" in wet.state_dict()
