@@ -404,7 +404,7 @@ class MultiTowerModel(nn.Module):
 # --------------------------------------------------------------------------------------------
 class MultiTaskModel(nn.Module):
     """Two towers -> in-batch retrieval loss and [u || i] -> DCN -> rating / CTR heads. tower_dropout:
-    MultiTowerModel's, drawn by compute_loss(training=True)."""
+    MultiTowerModel's, drawn by compute_loss(training=True) (training=None: by the module's mode)."""
 
     def __init__(self, config: ModelConfig, user_vocab: List[str], item_vocab: List[str],
                  feature_specs: Dict[str, Any], class_weights: Dict[int, float] = None,
@@ -487,8 +487,9 @@ class MultiTaskModel(nn.Module):
     def _compute_loss(self, data, training, return_parts, with_regularization):
         features, labels = self._split(data)
         ids = None
-        # (towers with dropout give equal ids different rows: no grouping by id)
-        wet = getattr(self.encoder, "tower_dropout", 0.0) > 0 and training
+        # (towers that drop give equal ids different rows: no grouping by id)
+        towers = [getattr(self.encoder, n, None) for n in ("user_tower", "item_tower")]
+        wet = any(t.drops(training) for t in towers if isinstance(t, Tower))
         if "user_id" in features and "movie_id" in features and not wet:
             # the towers see only the ids (:85-90), so equal ids give equal embeddings: the
             # retrieval loss's deduplicated pair groups rows by id (functional.inbatch_dedup_plan)

@@ -168,3 +168,32 @@ def test_a_model_with_dropout_is_served(tmp_path, monkeypatch):
     svc.load()
     # the generators stay in the model's own state
     assert "encoder.user_tower.dropouts.0.state" in wet.state_dict()
+
+
+def test_rows_are_not_grouped_by_id_where_the_towers_drop(monkeypatch):
+    """compute_loss takes `training` as the towers do: None is the module's mode."""
+    models, cfgm = pkg("models"), pkg("config")
+    cfg = cfgm.ModelConfig(embedding_dim=16, user_tower_dims=[8], item_tower_dims=[8], dnn_dims=[8])
+    B = 4
+    batch = ({"user_id": torch.zeros(B, dtype=torch.int64), "movie_id": torch.ones(B, dtype=torch.int64)},
+             {"rating": torch.zeros(B)})
+    seen = []
+
+    class Stop(Exception):
+        pass
+
+    class Cross:
+        @staticmethod
+        def apply(u, i, w, b, prec, ids):
+            seen[-1] += (ids is not None,)
+            raise Stop
+
+    monkeypatch.setattr(models, "RetrievalCrossFn", Cross)
+    for rate, grouped in ((0.5, {(True, None): False, (True, True): False, (True, False): True,
+                                 (False, None): True, (False, True): False}), (0.0, {(True, None): True, (True, True): True})):
+        m = models.MultiTaskModel(cfg, ["a"], ["b"], {}, device="cpu", tower_dropout=rate)
+        monkeypatch.setattr(m, "_towers", lambda f, orders=None, training=None: (seen.append((training,)), (None, None))[1])
+        for (mode, training), want in grouped.items():
+            with pytest.raises(Stop):
+                m.train(mode).compute_loss(batch, training=training)
+            assert seen[-1] == (training, want), (rate, mode, training)
