@@ -144,6 +144,8 @@ class Tower(nn.Module):
     def __init__(self, in_dim: int, dims: List[int], out_dim: int, seed: int = 0, device=None,
                  dropout_rate: float = 0.0):
         super().__init__()
+        if not 0.0 <= dropout_rate < 1.0:
+            raise ValueError(f"dropout rate must lie in [0, 1), got {dropout_rate!r}")
         layers = []
         prev = in_dim
         for j, u in enumerate(list(dims)):

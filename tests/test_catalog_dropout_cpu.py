@@ -197,3 +197,15 @@ def test_rows_are_not_grouped_by_id_where_the_towers_drop(monkeypatch):
             with pytest.raises(Stop):
                 m.train(mode).compute_loss(batch, training=training)
             assert seen[-1] == (training, want), (rate, mode, training)
+
+
+@pytest.mark.parametrize("rate", [-0.5, 1.0, float("nan")])
+def test_towers_refuse_what_dropout_refuses(rate):
+    models, cfgm = pkg("models"), pkg("config")
+    cfg = cfgm.ModelConfig(embedding_dim=16, user_tower_dims=[8], item_tower_dims=[8], dnn_dims=[8])
+    with pytest.raises(ValueError, match="rate"):
+        models.Tower(8, [16], 4, device="cpu", dropout_rate=rate)
+    with pytest.raises(ValueError, match="rate"):
+        models.MultiTowerModel(cfg, ["a"], ["b"], {}, device="cpu", tower_dropout=rate)
+    with pytest.raises(ValueError, match="rate"):
+        models.MultiTaskModel(cfg, ["a"], ["b"], {}, device="cpu", tower_dropout=rate)
