@@ -14,6 +14,7 @@ import weakref
 from typing import List, Optional, Sequence, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native
 from ._native import call, query
@@ -2406,8 +2407,11 @@ class CatalogSoftmaxFn(torch.autograd.Function):
 def catalog_softmax_loss(X, W, labels, scale: float = 1.0, weights=None, ignore_index: int = -100,
                          reduction: str = "sum"):
     """(loss, row_loss) of catalog_softmax_fwd, differentiable by X and W through the loss (not by the
-    weights). With gradients disabled the loss alone is formed (want_grad=False)."""
-    if not torch.is_grad_enabled():   # (a node is not told: its needs_input_grad are the inputs' requires_grad)
+    weights), in reverse mode; forward mode raises. With gradients disabled the loss alone is formed
+    (want_grad=False)."""
+    # (a node is not told of disabled gradients: its needs_input_grad are the inputs' requires_grad. Forward mode, which
+    # no_grad leaves on, is the node's to refuse)
+    if not torch.is_grad_enabled() and all(t is None or forward_ad.unpack_dual(t).tangent is None for t in (X, W, weights)):
         return _catalog_fwd(X.contiguous(), W.contiguous(), labels.contiguous(), scale,
                             weights.contiguous() if weights is not None else None, ignore_index, reduction,
                             False, False)[:2]

@@ -209,3 +209,25 @@ def test_towers_refuse_what_dropout_refuses(rate):
         models.MultiTowerModel(cfg, ["a"], ["b"], {}, device="cpu", tower_dropout=rate)
     with pytest.raises(ValueError, match="rate"):
         models.MultiTaskModel(cfg, ["a"], ["b"], {}, device="cpu", tower_dropout=rate)
+
+
+def test_forward_mode_is_refused(monkeypatch):
+    """A tangent is refused, with gradients enabled or not (no_grad leaves forward mode on), and never lost."""
+    F = pkg("functional")
+    from torch.autograd import forward_ad
+
+    def fwd(X, W, labels, scale, weights, ignore_index, reduction, want_grad, want_lse):
+        st = F.CatalogSoftmaxState(torch.empty(1), X.shape[0], W.shape[0], X.shape[1], X.dtype, scale, 0, 256)
+        return torch.zeros(()), torch.zeros(X.shape[0]), None, st
+
+    monkeypatch.setattr(F, "_catalog_fwd", fwd)
+    x, w, a = torch.zeros((3, 8)), torch.zeros((5, 8)), torch.ones(3)
+    y = torch.zeros(3, dtype=torch.int64)
+    for grad in (True, False):
+        with torch.set_grad_enabled(grad), forward_ad.dual_level():
+            for dual in ("x", "w", "a"):
+                t = {"x": x, "w": w, "a": a}
+                t[dual] = forward_ad.make_dual(t[dual], torch.ones_like(t[dual]))
+                with pytest.raises(NotImplementedError):
+                    F.catalog_softmax_loss(t["x"], t["w"], y, weights=t["a"])
+            F.catalog_softmax_loss(x, w, y, weights=a)
