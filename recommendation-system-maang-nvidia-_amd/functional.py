@@ -1522,6 +1522,7 @@ def dropout_ticket(state: torch.Tensor) -> torch.Tensor:
     with _on(state) as stream:
         ticket = torch.empty(2, dtype=torch.int64, device=state.device)
         call("rs_dropout_ticket", state.data_ptr(), ticket.data_ptr(), stream)
+    torch.autograd.graph.increment_version(state)   # a graph that saved the state as a ticket has lost it
     return ticket
 
 
@@ -1536,7 +1537,10 @@ def dropout_apply(x: torch.Tensor, rate: float, ticket: torch.Tensor, out: Optio
         raise ValueError("dropout: x and ticket must be on one device")
     if out is not None and (_dev(out, "out", x.dtype).shape != x.shape or out.device != x.device):
         raise ValueError("dropout: out must match x")
-    return _dropout(x, rate, ticket, out)
+    y = _dropout(x, rate, ticket, out)
+    if out is not None:
+        torch.autograd.graph.increment_version(out)
+    return y
 
 
 def _dropout(x, rate, ticket, out=None):
@@ -2437,7 +2441,8 @@ class DropoutFn(torch.autograd.Function):
 
 
 def dropout(x: torch.Tensor, rate: float, ticket: torch.Tensor) -> torch.Tensor:
-    """Dropout of x with the mask of `ticket` (dropout_ticket, or an int64 [2] (seed, step) tensor)."""
+    """Dropout of x with the mask of `ticket` (dropout_ticket, or an int64 [2] (seed, step) tensor that keeps its
+    values until the backward: one that was written in between is refused there)."""
     if not 0.0 <= rate < 1.0:
         raise ValueError(f"dropout: rate must lie in [0, 1), got {rate!r}")
     return DropoutFn.apply(x, float(rate), ticket)

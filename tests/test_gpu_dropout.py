@@ -184,3 +184,29 @@ def test_refusals(cuda):
         v = x.clone().requires_grad_(True)
         g, = torch.autograd.grad(F.dropout(v, 0.5, t).sum(), (v,), create_graph=True)
         g.sum().backward()
+
+
+def test_what_a_kernel_writes_counts_as_written(cuda):
+    """A generator used as its own ticket and then advanced, or an activation that dropout wrote over, is refused by the
+    backward that needs what they held."""
+    F = pkg("functional")
+    state = F.dropout_state(3, "cuda")
+    x = torch.randn((16, 8), device="cuda", requires_grad=True)
+    y = F.dropout(x, 0.5, state)
+    F.dropout_ticket(state)
+    with pytest.raises(RuntimeError, match="inplace"):
+        y.sum().backward()
+    F.dropout(x, 0.5, state).sum().backward()   # not advanced in between: its own mask
+    assert torch.equal(x.grad.cpu(), 2.0 * kept(x.shape, 0.5, 3, 1))
+    e = torch.exp(x)
+    F.dropout_apply(e.detach(), 0.5, ticket(1, 2), out=e.detach())
+    with pytest.raises(RuntimeError, match="inplace"):
+        e.sum().backward()
+    # the module's tickets are copies: two calls before a backward
+    drop = pkg("models").Dropout(0.5, seed=9, device="cuda")
+    a, b = drop(x), drop(x)
+    x.grad = None
+    (a + 2 * b).sum().backward()
+    assert torch.equal(x.grad.cpu(), 2.0 * kept(x.shape, 0.5, 9, 0) + 4.0 * kept(x.shape, 0.5, 9, 1))
+    with torch.inference_mode():
+        F.dropout_apply(torch.ones(8, device="cuda"), 0.5, F.dropout_ticket(F.dropout_state(3, "cuda")))
