@@ -65,16 +65,17 @@ enum { CS_LSE2 = 0, CS_KX = 1, CS_LAB = 2, CS_LQ = 3 };
 constexpr int CS_XREF = 13;
 __host__ __device__ inline int64_t cs_stat(int64_t n, int a) { return (n >> 5) * 128 + a * 32 + (n & 31); }
 
-// fp32: an item's scale 2^e, per 32 items two arrays of 32 words: f = 2^(-e - 1), the factor of its scores and
-// of its exponentials in the row pass's second product, and -log2 f. e = 3 + 8 i brings the item's largest entry
-// into [2^6, 2^14) (i = 1: entries from 2^-5 to 2^3): neighbours mostly share it, and what they share costs no work
-// per score (row pass of 4096 x 20k x 64: 95 us with one scale, 103 with items over 16 binades; 8192 x 100k x 128: 0.98
-// ms and 0.99). An item with an entry that is not finite has 2^90 and infinity (NaN, if one of them is), and +-2^14
-// for its infinite entries, zeros for the others. e is at most 99 (2^-27 for the smallest normal number): an
-// exponential in the row pass stays between 2^-101 (the row's likeliest item) and 2^115.
-enum { CS_WF = 0, CS_WE = 1 };
-constexpr int CS_WE_MAX = 99;
-__host__ __device__ inline int64_t cs_wstat(int64_t v, int a) { return (v >> 5) * 64 + a * 32 + (v & 31); }
+// fp32: an item's scale 2^e, per 32 items three arrays of 32 words: f = 2^(-e - 1), the factor of its scores;
+// -log2 f; and 2^15 f, the factor of its exponentials in the row pass's second product. e = 3 + 8 i brings the
+// item's largest entry into [2^6, 2^14) (i = 1: entries from 2^-5 to 2^3): neighbours mostly share it, and what they
+// share costs no work per score (row pass of 4096 x 20k x 64: 95 us with one scale, 103 with items over 16 binades;
+// 8192 x 100k x 128: 0.98 ms and 0.99). An item with an entry that is not finite has f = 2^90 and infinity (NaN, if one
+// of them is) for -log2 f, and +-2^14 for its infinite entries, zeros for the others. e lies between -113 (2^15 for
+// the largest number) and 99 (2^-27 for the smallest normal one): the row pass's exponentials of a row's likeliest
+// item stay between 2^-112 and 2^100.
+enum { CS_WF = 0, CS_WE = 1, CS_WP = 2 };
+constexpr int CS_WE_MIN = -113, CS_WE_MAX = 99;
+__host__ __device__ inline int64_t cs_wstat(int64_t v, int a) { return (v >> 5) * 96 + a * 32 + (v & 31); }
 
 struct CsPass {
   const char* R;          // resident rows [nR][D] (plane stride r_plane bytes)
@@ -232,7 +233,7 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
   constexpr int UB = cs_cfg(D, NP, MODE).UB, NW = cs_cfg(D, NP, MODE).NW, KT = cs_cfg(D, NP, MODE).KT;
   constexpr int NB = cs_cfg(D, NP, MODE).NB;
   constexpr int ROWB = 2 * D, PLANE = KT * ROWB, IMG = NP * PLANE, NDT = D / 16, NC = D / 32;
-  constexpr int SROW = MODE == CS_COL ? 16 : NP == 2 ? 8 : 0;  // bytes of statistics per streamed row
+  constexpr int SROW = MODE == CS_COL ? 16 : NP == 2 ? 12 : 0;  // bytes of statistics per streamed row
   constexpr int STAT = KT * SROW, BUF = IMG + STAT;
   constexpr bool RUNMAX = MODE != CS_COL || NP == 2;
   __shared__ __attribute__((aligned(1024))) char smem[NB * BUF];
@@ -339,7 +340,7 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
     for (int ub = 0; ub < UB; ++ub) same &= !__any(kq[ub] != f0);
   }
   const float kw = p.kbase;
-  const float ps = NP == 2 ? CS_PS : 0.f;
+  const float ps = NP == 2 && MODE == CS_COL ? CS_PS : 0.f;  // (the row pass's items bring it)
   const bool flip = MODE == CS_COL && p.scal->neg;
 
   // row reads: A row i16 of subtile kb = row 8 (i16 / 4) + 4 kb + i16 % 4 of 32, chunk 4 c + g
@@ -549,7 +550,7 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
       if constexpr (NP == 2) {
         // the items' scales: one for the group, or one each (then in the scores, the group's being 1)
         const int ll = ln & (32 * SG - 1);
-        const float we = cs_lds<float>(st + (ll >> 5) * 256 + CS_WE * 128 + (ll & 31) * 4);
+        const float we = cs_lds<float>(st + (ll >> 5) * (32 * SROW) + CS_WE * 128 + (ll & 31) * 4);
         e0 = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, we)));
         one = e0 < INFINITY && !__any(!(we == e0));
         if (!one) {
@@ -665,7 +666,7 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
     const int k = i / UB, ub = i % UB;
     f32x4 ls, e, f = {};
     if constexpr (MODE == CS_COL && NP == 1) ls = cs_lds<f32x4>(stat_at(sg, CS_LSE2, k));
-    if constexpr (MODE == CS_ROW && NP == 2) f = cs_lds<f32x4>(stat_at(sg, CS_WF, k));
+    if constexpr (MODE == CS_ROW && NP == 2) f = cs_lds<f32x4>(stat_at(sg, CS_WP, k));
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const float x = s.v[k][ub][r];
@@ -992,6 +993,7 @@ __global__ __launch_bounds__(256) void cs_image_kernel(CsImage p) {
         if (c == 0) p.kx[r] = ldexpf(1.f, -e);
       } else {
         e = !(a > 0.f) || e > CS_WE_MAX ? CS_WE_MAX : ((e - 3) & ~7) + 3;
+        e = e < CS_WE_MIN ? CS_WE_MIN : e;
         int odd = 0;  // 1: an infinite entry, 2: a NaN
         for (int j = 0; j < 4; ++j) odd = isnan(v[j]) ? 2 : isinf(v[j]) && odd < 1 ? 1 : odd;
 #pragma unroll
@@ -1006,6 +1008,7 @@ __global__ __launch_bounds__(256) void cs_image_kernel(CsImage p) {
         if (c == 0) {
           p.wstat[cs_wstat(r, CS_WF)] = odd ? 0x1p90f : ldexpf(1.f, -e - 1);
           p.wstat[cs_wstat(r, CS_WE)] = odd == 2 ? NAN : odd ? INFINITY : (float)(e + 1);
+          p.wstat[cs_wstat(r, CS_WP)] = ldexpf(1.f, 14 - e);
         }
         if (r >= rows) continue;  // past the last item: statistics alone
       }
@@ -1194,7 +1197,7 @@ __device__ __forceinline__ void cs_row(const CsRows& p) {
   // statistic takes a finite score out, not an infinite one; fp32's scores are of scaled values)
   if (NP == 1 && p.stat && lb < 0 && lane < LPR) *reinterpret_cast<u32x2*>(p.ximg + n * (2 * DP) + 2 * c) = u32x2{0, 0};
   if (!p.dx || lane >= LPR) return;
-  const double il = L == 0. ? 0. : (NP == 2 ? 2. : 1.) / L;  // fp32: O holds half its items (f = 2^(-e - 1)); L may pass fp32's range
+  const double il = L == 0. ? 0. : (NP == 2 ? 0x1p-14 : 1.) / L;  // fp32: O holds 2^14 times its items; L may pass fp32's range
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     if (c + j >= p.D) continue;
@@ -1365,7 +1368,7 @@ struct CsKeep {
     wimg = s.wimage ? c.take<char>((size_t)s.V * s.DP * 2 * s.NP) : nullptr;
     lab = c.take<int32_t>(s.Npad);
     kx = c.take<float>(s.Npad);
-    wstat = s.wimage && s.NP == 2 ? c.take<float>(s.Vpad * 2) : nullptr;
+    wstat = s.wimage && s.NP == 2 ? c.take<float>(s.Vpad * 3) : nullptr;
     stat = c.take<float>(s.Npad * 4);
     dx = want & RS_CATALOG_DX ? c.take<float>((size_t)s.N * s.D) : nullptr;
     bytes = align_up(c.off, 256);

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from conftest import pkg
-from test_gpu_catalog import DTYPES, IGN, inputs, reference, step, tolerances, within
+from test_gpu_catalog import DTYPES, IGN, check, inputs, reference, step, tolerances, within
 
 pytestmark = pytest.mark.gpu
 
@@ -123,3 +123,13 @@ def test_infinite_and_nan_items(cuda):
         w2[9, 3] = float("nan")
         loss, row, dx, dw = step(x, w2, y)
         assert bool(row.isnan().all()) and bool(dx.isnan().all()) and bool(dw.isnan().all())
+
+
+@DTYPES
+@pytest.mark.parametrize("size", [2.0 ** -18, 2.0 ** -9, 1.0, 4.0])
+@pytest.mark.parametrize("N,V,D", [(1, 1, 1), (345, 2, 96), (90, 3, 64)])
+def test_few_items_of_any_size(cuda, dtype, N, V, D, size):
+    """One to three items: no other items' roundings average out those of a probability."""
+    x, w, y, _ = inputs(N, V, D, dtype, seed=N, ignored=0.7 if N > 1 else 0.0, scale=0.1)
+    check(x, (w.float() * size).to(dtype), y, None, 0.1)
+    check(x, (w.float() * size).to(dtype), torch.full_like(y, IGN), None, 0.1)
