@@ -812,15 +812,17 @@ int rs_l2_normalize_rows_f32(const float* x, int64_t n, int64_t D, float* out, r
  * weights a [N] (nullable: 1):
  *   s_nv = c <x_n, w_v>, lse_n = log sum_v exp s_nv, row_n = lse_n - s_n,label, loss = sum a_n row_n / Z,
  * Z = 1, or with `mean` the sum of a over the labelled rows (a sum of zero, or no labelled row: loss 0).
- * No logits are
- * stored. float32 operands are held as two fp16 terms under a power-of-two scale for each row of X and each
- * item: a logit's error is at most c (2^-20 sum_d |x_d w_d| + D 2^-30 max|x_n| max|w_v|) beside fp32 sums.
- * bfloat16 operands are exact; the gradients' probabilities are rounded to bfloat16. An item is masked by a
- * logit far below the others or of -infinity (one infinite entry of w against a finite one of x): the rest is
- * as without it, its row of dW zero; dX's column of an infinite entry has no value. A NaN entry, or a logit of
- * +infinity, makes its rows NaN. Where every logit of a row lies below -1e30 its loss has no value. An ignored row has row_loss 0, enters neither loss nor gradients (whatever its x holds) and
- * has the lse of its finite entries; a label that is neither in range nor ignore_index makes its row
- * loss, its dX row and the loss NaN and stays out of dW. row_loss, lse [N] (nullable) and *loss are fp32.
+ * No logits are stored. float32 operands are held as two fp16 terms under a power-of-two scale for each row
+ * of X and each item: a logit's error is at most c (2^-20 sum_d |x_d w_d| + D 2^-30 max|x_n| max|w_v|) beside
+ * fp32 sums. bfloat16 operands are exact; the gradients' probabilities are rounded to bfloat16.
+ * An item is masked by a logit far below the others, or of -infinity from one infinite entry of w against a
+ * finite, non-zero one of x (several in one item: in float32 the sign of their sum counts): the rest is as
+ * without it and its row of dW zero; dX's column of an infinite entry has no value. A NaN entry of w, zero
+ * times infinity and a logit of +infinity make their rows NaN. Where every logit of a row lies below -1e30 the
+ * row has no value.
+ * An ignored row has row_loss 0, enters neither loss nor gradients (whatever its x holds) and has the lse of
+ * its finite entries; a label that is neither in range nor ignore_index makes its row loss, its dX row and the
+ * loss NaN and stays out of dW. row_loss, lse [N] (nullable) and *loss are fp32.
  * want: RS_CATALOG_DX / _DW: which gradients a backward will be asked for (0: the loss alone, about
  * half the work). `keep` (rs_catalog_softmax_keep_bytes, same arguments) carries the forward's state to
  * the backward and is only read there; the workspace may be reused after each call. X, W, keep,
@@ -840,10 +842,10 @@ int rs_catalog_softmax_bwd(const void* W, int64_t N, int64_t V, int64_t D, int d
                            void* workspace, size_t workspace_bytes, rs_stream_t stream);
 
 /* ---- dropout ------------------------------------------------------------------------------------
- * keras.layers.Dropout (the reference's dropout_rate, src/config.py:21, src/models.py:16,22): y = x /
- * (1 - rate) where element i's word is at least round(rate 2^32), else 0. Words: Philox4x32-10 with key =
- * ticket[0] and counter (i / 4, ticket[1]), word i % 4; ticket is int64 [2] on the device. The backward is
- * the same call on dy with the same ticket. x and y hold n < 2^35 elements of dtype; y may be x.
+ * keras.layers.Dropout (the reference's dropout_rate, src/config.py:21, src/models.py:16,22): y = x f,
+ * f = 1 / (1 - rate) in fp32, where element i's word is at least round(rate 2^32), else 0. Words:
+ * Philox4x32-10 with key = ticket[0] and counter (i / 4, ticket[1]), word i % 4; ticket is int64 [2] on the
+ * device. The backward is the same call on dy with the same ticket. x and y hold n < 2^35 elements of dtype; y may be x.
  * rs_dropout_ticket copies state (int64 [2]: seed, step) to ticket and adds one to the step, on the
  * device, so a captured step draws a new mask at each replay. */
 int rs_dropout(const void* x, int64_t n, int dtype, double rate, const int64_t* ticket, void* y, rs_stream_t stream);

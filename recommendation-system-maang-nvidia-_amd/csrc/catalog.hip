@@ -180,11 +180,11 @@ enum { CS_STATS = 0, CS_ROW = 1, CS_COL = 2 };
 // Shape of a pass: UB 16-row subtiles of resident rows per wave, NW waves, tiles of KT streamed rows taken
 // in groups of 32 SG rows, NB tiles in LDS (the copies run NB - 1 tiles ahead), WG workgroups per CU.
 // O, the resident rows and a group's scores fill the registers. Groups of 64 rows form half as many sums
-// and maxima as groups of 32 (8192 x 100k x 128 fp32, row pass: 0.97 against 1.19 ms). Three waves a SIMD
-// where they fit: at 64 columns (8192 x 100k, fp32 passes 0.56 and 0.58 against 0.61 and 0.68 ms), and for
-// the bf16 column pass, without a running maximum, at groups of 32 (16384 x 1M x 128: 6.2 against 6.8 ms;
-// 4096 x 60k x 256: 260 against 315 us). At 256 columns a wave holds 16 rows: 32 leave one wave a SIMD
-// (4096 x 60k x 256 fp32: 852 and 751 against 748 and 676 us).
+// and maxima as groups of 32 (8192 x 100k x 128 fp32, forward: 0.97 against 1.19 ms). Three waves a SIMD
+// where they fit: at 64 columns (8192 x 100k fp32, forward and backward: 0.59 and 0.56 ms against 0.60 and 0.59
+// with two), and for the bf16 column pass, without a running maximum, at groups of 32 (16384 x 1M x 128: 6.2
+// against 6.8 ms; 4096 x 60k x 256: 260 against 315 us). At 256 columns a wave holds 16 rows: 32 leave one wave a
+// SIMD (4096 x 60k x 256 fp32: 697 and 727 against 641 and 632 us).
 struct CsCfg {
   int UB, NW, KT, NB, SG, WG;
 };
@@ -790,7 +790,8 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
 
 // ---- the loss alone, few fp32 rows -----------------------------------------------------------------
 // Up to 64 rows (256-wide: 32) against the catalogue: its bytes are the bound, so w is read once, as it lies (an image
-// would read it twice and write it), straight into the A operand of the fp32 matrix instruction (exact
+// would read it twice and write it; so do the widths whose rows do not start on 16 bytes, for whose loads this kernel
+// has no form), straight into the A operand of the fp32 matrix instruction (exact
 // products; 16 items x 4 columns x 16 rows each), one step of 16 items ahead. A workgroup's four waves
 // share a range of items; their maxima and sums join in LDS.
 struct CsFew {
@@ -1208,9 +1209,10 @@ __device__ __forceinline__ void cs_row(const CsRows& p) {
   }
 }
 
-// The rows, and up to CS_TAIL_ROWS of them the total in the grid's last workgroup: 3 to 6 us more than the
-// rows alone, a kernel of its own 4 to 5 and a launch of the host's time, which bounds such a step. Past
-// that the tickets cost more (4096 rows: 22 us against 13 + 5; 8192: 27 against 16 + 7).
+// The rows, and up to CS_TAIL_ROWS of them (one round of that workgroup's loads) the total in the grid's last
+// workgroup. Forwards of 3000 x 64 to 100,000 x 128 items replayed from a graph: 0 to 1 us more than with a kernel
+// of its own up to 2048 rows, 3 to 5 us more at 2500 and 4 to 13 at 8192. A call bound by the host gains its launch
+// (64 rows: 19 us against 22).
 constexpr int CS_TAIL_ROWS = 2048;
 template <int DP, int NP, int NWV>
 __global__ __launch_bounds__(NWV == 1 ? 256 : 64 * NWV) void cs_rows_kernel(CsRows p) {

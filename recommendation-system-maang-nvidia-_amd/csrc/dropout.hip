@@ -3,8 +3,8 @@
 //
 // Words: Philox4x32-10 (Salmon et al., "Parallel random numbers: as easy as 1, 2, 3", SC 2011), key =
 // the 64-bit seed, counter = (element / 4, step), word element % 4. Element i is kept iff its word is
-// at least round(rate 2^32): y = x / (1 - rate), one fp32 rounding (then one to bf16); a dropped
-// element is 0 whatever x holds there.
+// at least round(rate 2^32): y = x f, f = 1 / (1 - rate) rounded to fp32 and the product once more (then once
+// to bf16); a dropped element is 0 whatever x holds there.
 //
 // Bound: HBM, one read and one write per element.
 #include "split.hpp"
