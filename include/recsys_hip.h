@@ -818,8 +818,8 @@ int rs_l2_normalize_rows_f32(const float* x, int64_t n, int64_t D, float* out, r
  * An item is masked by a logit far below the others, or of -infinity from one infinite entry of w against a
  * finite, non-zero one of x (several in one item: in float32 the sign of their sum counts): the rest is as
  * without it and its row of dW zero; dX's column of an infinite entry has no value. A NaN entry of w, zero
- * times infinity and a logit of +infinity make their rows NaN. Where every logit of a row lies below -1e30 the
- * row has no value.
+ * times infinity and a logit of +infinity make their rows NaN, and so does a row whose every logit lies below
+ * -1e30.
  * An ignored row has row_loss 0, enters neither loss nor gradients (whatever its x holds) and has the lse of
  * its finite entries; a label that is neither in range nor ignore_index makes its row loss, its dX row and the
  * loss NaN and stays out of dW. row_loss, lse [N] (nullable) and *loss are fp32.

@@ -1174,7 +1174,9 @@ __device__ __forceinline__ void cs_row(const CsRows& p) {
 #pragma unroll
   for (int k = LPR / 2; k > 0; k >>= 1) sy += __shfl_xor(sy, k, 64);
   sy *= (double)p.scale * CS_LOG2E;
-  const float t = (float)((o2 - sy) * CS_LN2);
+  // every item, the label's too, below the running maximum's start: what they are to one another is lost
+  const bool lost = lb >= 0 && L == 0. && p.V > 1 && !(sy > 0.5 * CS_MIN);
+  const float t = lost ? NAN : (float)((o2 - sy) * CS_LN2);
   const float et = expf(-fabsf(t)), soft = log1pf(et);
   const float q = t > 0.f ? 1.f / (1.f + et) : et / (1.f + et);  // NaN stays NaN
   const double lse2 = lb >= 0 ? fmax(o2, sy) + (double)soft * CS_LOG2E : o2;
@@ -1187,8 +1189,11 @@ __device__ __forceinline__ void cs_row(const CsRows& p) {
     const bool live = lb >= 0;
     double ca = log2f(fabsf(a));
     if (NP == 2) ca += ilogbf(p.kx[n]) + CS_XREF;
-    // NaN statistics of a labelled row reach every item's gradient, as the formula's do
-    p.stat[cs_stat(n, CS_LSE2)] = live ? (float)(lse2 - ca) : INFINITY;
+    // NaN statistics of a labelled row reach every item's gradient, as the formula's do; infinite is the statistic of a
+    // weight of zero alone
+    double ls = lse2 == INFINITY ? NAN : lse2 - ca;
+    if (a != 0.f && !isnan(ls)) ls = fmin(fmax(ls, -(double)FLT_MAX), (double)FLT_MAX);
+    p.stat[cs_stat(n, CS_LSE2)] = live ? (float)ls : INFINITY;
     // (a row that takes no part: a factor whose product with any score is finite)
     p.stat[cs_stat(n, CS_KX)] = NP == 2 && live ? fminf(fmaxf(2.f * p.kbase * p.kx[n], FLT_MIN), FLT_MAX) : 1.f;
     reinterpret_cast<int32_t*>(p.stat)[cs_stat(n, CS_LAB)] = live ? 2 * lb + (a < 0.f) : lb;
@@ -1203,7 +1208,8 @@ __device__ __forceinline__ void cs_row(const CsRows& p) {
   for (int j = 0; j < 4; ++j) {
     if (c + j >= p.D) continue;
     float v = 0.f;
-    if (lb >= 0) v = L == 0. ? 0.f : a * q * (NP == 2 ? (float)(o[j] * il) - wv[j] : o[j] * (float)il - wv[j]);
+    if (lost) v = NAN;
+    else if (lb >= 0) v = L == 0. ? 0.f : a * q * (NP == 2 ? (float)(o[j] * il) - wv[j] : o[j] * (float)il - wv[j]);
     else if (lb == -2) v = NAN;
     p.dx[n * p.D + c + j] = v;
   }

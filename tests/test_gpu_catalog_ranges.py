@@ -133,3 +133,24 @@ def test_few_items_of_any_size(cuda, dtype, N, V, D, size):
     x, w, y, _ = inputs(N, V, D, dtype, seed=N, ignored=0.7 if N > 1 else 0.0, scale=0.1)
     check(x, (w.float() * size).to(dtype), y, None, 0.1)
     check(x, (w.float() * size).to(dtype), torch.full_like(y, IGN), None, 0.1)
+
+
+@DTYPES
+@pytest.mark.parametrize("bias", [-1e32, -3.3e38, -float("inf")])
+@pytest.mark.parametrize("N", [40, 130])
+def test_rows_whose_items_are_all_masked(cuda, dtype, bias, N):
+    """Nothing is left to compare the label with: NaN, never a loss of zero; a single item is certain whatever its
+    finite logit; a label far above the others, which are masked, is certain too."""
+    F = pkg("functional")
+    x, w, y, _ = inputs(N, 300, 64, dtype, seed=N)
+    x[:, -1] = 1.0
+    w[:, -1] = bias
+    loss, row, dx, dw = step(x, w, y)
+    assert all(bool(t.isnan().all()) for t in (loss, row, dx))
+    assert bool(F.catalog_softmax_fwd(x, w, y, want_grad=False)[1].isnan().all())
+    if bias > -float("inf"):
+        loss, row, dx, dw = step(x, w[:1].contiguous(), torch.zeros_like(y))
+        assert not any(bool(t.any()) for t in (loss, row, dx, dw))
+    w[7, -1] = 0.0
+    loss, row, dx, dw = step(x, w, torch.full_like(y, 7))
+    assert not any(bool(t.any()) for t in (loss, row, dx[:, :-1], dw))
