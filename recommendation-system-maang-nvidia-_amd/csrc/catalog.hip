@@ -71,10 +71,13 @@ __host__ __device__ inline int64_t cs_stat(int64_t n, int a) { return (n >> 5) *
 // share costs no work per score (row pass of 4096 x 20k x 64: 95 us with one scale, 103 with items over 16 binades;
 // 8192 x 100k x 128: 0.98 ms and 0.99). An item with an entry that is not finite has f = 2^90 and infinity (NaN, if one
 // of them is) for -log2 f, and +-2^14 for its infinite entries, zeros for the others. e lies between -113 (2^15 for
-// the largest number) and 99 (2^-27 for the smallest normal one): the row pass's exponentials of a row's likeliest
-// item stay between 2^-112 and 2^100.
+// the largest number) and 99 (2^-27 for the smallest normal one). The row pass's exponentials are 2^(s - m - e0), m
+// the running maximum of s + log2 f, e0 a group's -log2 f where its items share it, up to 28 (most exponentials are at
+// most 1 then, and round as little as can be), else the common window's 12 or, with an item of 2^115 and more, zero: a
+// row's likeliest item stays within 2^-124 and 2^100.
 enum { CS_WF = 0, CS_WE = 1, CS_WP = 2 };
 constexpr int CS_WE_MIN = -113, CS_WE_MAX = 99;
+constexpr float CS_WE_REF = 12.f, CS_WE_FAR = 28.f, CS_WE_BIG = -100.f;
 __host__ __device__ inline int64_t cs_wstat(int64_t v, int a) { return (v >> 5) * 96 + a * 32 + (v & 31); }
 
 struct CsPass {
@@ -495,11 +498,11 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
   // Before a group's exponentials (its first streamed row is n0): the label's term leaves them and the
   // running maximum is raised (up, al: what that multiplies O and l by). Both are rare, and what they
   // change is small, so the common path has no branch between its matrix and vector instructions.
-  auto prepare = [&](int64_t n0, int ln, uint32_t st, uint32_t sg, Scores& s, float (&al)[UB], float (&kg)[UB], bool& up, bool& hit)
-      __attribute__((always_inline)) {
+  auto prepare = [&](int64_t n0, int ln, uint32_t st, uint32_t sg, Scores& s, float (&al)[UB], float (&kg)[UB], float& e0, bool& up,
+                     bool& hit) __attribute__((always_inline)) {
     up = hit = false;
     bool one = true;
-    float e0 = 0.f;
+    float ew = 0.f;  // -log2 f of the group's items, where they share it
     if constexpr (MODE == CS_COL) {
       if constexpr (NP == 2) {
         // log2 p = s k_n f_v - lse2_n (s k_n first: that is finite in a row that takes no part, which has k_n = 1)
@@ -555,7 +558,7 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
         one = e0 < INFINITY && !__any(!(we == e0));
         if (!one) {
           asm volatile("");  // keeps the rare path a branch
-          e0 = 0.f;
+          e0 = __any(we < CS_WE_BIG) ? 0.f : CS_WE_REF;
 #pragma unroll
           for (int k = 0; k < 2 * SG; ++k) {
             const f32x4 f = cs_lds<f32x4>(stat_at(sg, CS_WF, k)), w = cs_lds<f32x4>(stat_at(sg, CS_WE, k));
@@ -569,7 +572,9 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
               }
           }
         }
-        const float f0 = __builtin_bit_cast(float, (127 - (int)e0) << 23);
+        const float f0 = one ? __builtin_bit_cast(float, (127 - (int)e0) << 23) : 1.f;
+        ew = e0;
+        if (one) e0 = fminf(e0, CS_WE_FAR);
 #pragma unroll
         for (int ub = 0; ub < UB; ++ub) kg[ub] = fminf(fmaxf(kq[ub] * f0, FLT_MIN), FLT_MAX);
       }
@@ -603,7 +608,7 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
         for (int k = 0; k < 2 * SG; ++k)
 #pragma unroll
           for (int r = k == 0 ? 2 : 0; r < 4; r += 2) z = fmaxf(fmaxf(s.v[k][ub][r], s.v[k][ub][r + 1]), z);
-        mx[ub] = MODE == CS_COL ? z : NP == 1 ? z * kq[ub] : __builtin_fmaf(z, kg[ub], -e0);
+        mx[ub] = MODE == CS_COL ? z : NP == 1 ? z * kq[ub] : __builtin_fmaf(z, kg[ub], -ew);
       }
       if constexpr (MODE != CS_COL && NP == 2)  // the maximum is that of exp s times the item's factor
         if (!one) {
@@ -630,6 +635,7 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
         for (int ub = 0; ub < UB; ++ub) {
           float x = fmaxf(mx[ub], __shfl_xor(mx[ub], 16, 64));
           x = fmaxf(x, __shfl_xor(x, 32, 64));
+          if (MODE != CS_COL && NP == 2) x = ceilf(x);  // m + e0 is exact
           x = fmaxf(x, m[ub]);
           al[ub] = __builtin_amdgcn_exp2f(m[ub] - x);
           l[ub] *= cs_exp2_d<NP>(m[ub] - x);
@@ -661,16 +667,16 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
     }
   };
   // exponentials of part i = (subtile k, ub) of 2 SG UB
-  auto exponentials = [&](int i, uint32_t sg, const Scores& s, Probs& pb, const float (&kg)[UB], float (&sum)[UB])
-      __attribute__((always_inline)) {
+  auto exponentials = [&](int i, uint32_t sg, const Scores& s, Probs& pb, const float (&kg)[UB], const float (&mg)[UB], float p0,
+                          float (&sum)[UB]) __attribute__((always_inline)) {
     const int k = i / UB, ub = i % UB;
     f32x4 ls, e, f = {};
     if constexpr (MODE == CS_COL && NP == 1) ls = cs_lds<f32x4>(stat_at(sg, CS_LSE2, k));
-    if constexpr (MODE == CS_ROW && NP == 2) f = cs_lds<f32x4>(stat_at(sg, CS_WP, k));
+    if constexpr (MODE == CS_ROW && NP == 2) f = cs_lds<f32x4>(stat_at(sg, CS_WP, k)) * p0;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const float x = s.v[k][ub][r];
-      if constexpr (MODE != CS_COL) e[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x, NP == 2 ? kg[ub] : kq[ub], -m[ub]));
+      if constexpr (MODE != CS_COL) e[r] = __builtin_amdgcn_exp2f(NP == 2 ? __builtin_fmaf(x, kg[ub], -mg[ub]) : __builtin_fmaf(x, kq[ub], -m[ub]));
       else if constexpr (NP == 2) e[r] = __builtin_amdgcn_exp2f(x - m[ub]);
       else e[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x, kw, -ls[r]));
     }
@@ -707,18 +713,21 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
         if constexpr (NP == 2) asm volatile("" : "+v"(ln));
         uint32_t sg = st + 32 * (ln >> 4);
         if constexpr (NP == 2) asm("" : "+v"(sg));
-        float al[UB], kg[UB], sum[UB] = {};
+        float al[UB], kg[UB], mg[UB], sum[UB] = {}, e0 = 0.f;
         bool up, hit;
         Scores s;
         Probs pb;
         scores(ln, bo, s);
-        prepare(n0, ln, st, sg, s, al, kg, up, hit);
+        prepare(n0, ln, st, sg, s, al, kg, e0, up, hit);
+        const float p0 = __builtin_bit_cast(float, (127 + (int)e0) << 23);
+#pragma unroll
+        for (int ub = 0; ub < UB; ++ub) mg[ub] = m[ub] + e0;
         rescale(up, al);
 #pragma unroll
-        for (int i = 0; i < 2 * SG * UB; ++i) exponentials(i, sg, s, pb, kg, sum);
+        for (int i = 0; i < 2 * SG * UB; ++i) exponentials(i, sg, s, pb, kg, mg, p0, sum);
         if constexpr (MODE != CS_COL)
 #pragma unroll
-          for (int ub = 0; ub < UB; ++ub) l[ub] += (double)sum[ub];
+          for (int ub = 0; ub < UB; ++ub) l[ub] += NP == 2 ? (double)sum[ub] * (double)p0 : (double)sum[ub];
         if constexpr (MODE == CS_COL) {
           if (hit) {
             asm volatile("");  // keeps the rare path a branch
@@ -974,9 +983,9 @@ __global__ __launch_bounds__(256) void cs_image_kernel(CsImage p) {
       *reinterpret_cast<u32x2*>(dst + r * (2 * DP) + 2 * c) =
           u32x2{h[0] | ((uint32_t)h[1] << 16), h[2] | ((uint32_t)h[3] << 16)};
     } else {
-      const float* s = (const float*)src + r * p.D + c;
+      const float* s = (const float*)src + (is_x || r < rows ? r : rows - 1) * p.D + c;
       f32x4 v = {0.f, 0.f, 0.f, 0.f};
-      if (r < rows) {
+      if (!is_x || r < rows) {
         if (vec) {
           if (c < p.D) v = *reinterpret_cast<const f32x4*>(s);
         } else {
@@ -1011,7 +1020,7 @@ __global__ __launch_bounds__(256) void cs_image_kernel(CsImage p) {
           p.wstat[cs_wstat(r, CS_WE)] = odd == 2 ? NAN : odd ? INFINITY : (float)(e + 1);
           p.wstat[cs_wstat(r, CS_WP)] = ldexpf(1.f, 14 - e);
         }
-        if (r >= rows) continue;  // past the last item: statistics alone
+        if (r >= rows) continue;  // past the last item: its statistics again, so that its group keeps one scale
       }
       const float sc = ldexpf(1.f, e);
       uint32_t h[2], lo[2];

@@ -154,3 +154,11 @@ def test_rows_whose_items_are_all_masked(cuda, dtype, bias, N):
     w[7, -1] = 0.0
     loss, row, dx, dw = step(x, w, torch.full_like(y, 7))
     assert not any(bool(t.any()) for t in (loss, row, dx[:, :-1], dw))
+
+
+@DTYPES
+@pytest.mark.parametrize("N,D,scale,size", [(2404, 1, 0.1, 2.0 ** -10), (94, 100, 14.3, 2.0 ** -16), (300, 33, 1.0, 2.0 ** -20)])
+def test_an_only_item(cuda, dtype, N, D, scale, size):
+    """The log sum of a catalogue of one item is its logit, to the roundings of the terms alone."""
+    x, w, y, _ = inputs(N, 1, D, dtype, seed=N, ignored=0.5, scale=scale)
+    check(x, (w.float() * size).to(dtype), y, None, scale)
