@@ -814,7 +814,8 @@ int rs_l2_normalize_rows_f32(const float* x, int64_t n, int64_t D, float* out, r
  * Z = 1, or with `mean` the sum of a over the labelled rows (a sum of zero, or no labelled row: loss 0).
  * No logits are stored. float32 operands are held as two fp16 terms under a power-of-two scale for each row
  * of X and each item: a logit's error is at most c (2^-20 sum_d |x_d w_d| + D 2^-30 max|x_n| max|w_v|) beside
- * fp32 sums. bfloat16 operands are exact; the gradients' probabilities are rounded to bfloat16.
+ * fp32 sums. bfloat16 operands are exact; in the gradients the probabilities, but the
+ * label's own, are rounded to bfloat16.
  * An item is masked by a logit far below the others, or of -infinity from one infinite entry of w against a
  * finite, non-zero one of x (several in one item: in float32 the sign of their sum counts): the rest is as
  * without it and its row of dW zero; dX's column of an infinite entry has no value. A NaN entry of w, zero

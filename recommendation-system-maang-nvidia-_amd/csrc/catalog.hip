@@ -17,7 +17,10 @@
 // difference of nearly equal numbers where the label is nearly certain. The column pass takes -q for
 // the label's element.
 //
-// bf16 inputs: one bf16 product, p rounded to bf16 (2^-8 of each term, as its output is). fp32 inputs:
+// bf16 inputs: one bf16 product, p rounded to bf16 (2^-8 of each term, as its output is; a p in two terms would be
+// half as much matrix work again in each pass). The label's term keeps fp32's precision: dx has w_y itself, the column
+// pass a second product of what -q's rounding lost, in the groups of rows that hold a label of the wave's items
+// (16384 x 1M x 128: none in a thousand; 1021 x 50k x 96: 49 -> 54 us). fp32 inputs:
 // every operand as two fp16 terms h + l of the value scaled by a power of two (|x - h - l| <= 2^-22
 // |x|, or 2^-39 of the scale's largest value), three products h h, h l, l h per fp32 product: half the
 // matrix work of the exact three-term bf16 split. Every row of x and every item has a scale of its own, so
@@ -68,8 +71,8 @@ __host__ __device__ inline int64_t cs_stat(int64_t n, int a) { return (n >> 5) *
 // fp32: an item's scale 2^e, per 32 items three arrays of 32 words: f = 2^(-e - 1), the factor of its scores;
 // -log2 f; and 2^15 f, the factor of its exponentials in the row pass's second product. e = 3 + 8 i brings the
 // item's largest entry into [2^6, 2^14) (i = 1: entries from 2^-5 to 2^3): neighbours mostly share it, and what they
-// share costs no work per score (row pass of 4096 x 20k x 64: 95 us with one scale, 103 with items over 16 binades;
-// 8192 x 100k x 128: 0.98 ms and 0.99). An item with an entry that is not finite has f = 2^90 and infinity (NaN, if one
+// share costs no work per score (forward of 4096 x 20k x 64: 98 us with one scale, 106 with items over 16 binades;
+// 8192 x 100k x 128: 1.03 ms and 1.02). An item with an entry that is not finite has f = 2^90 and infinity (NaN, if one
 // of them is) for -log2 f, and +-2^14 for its infinite entries, zeros for the others. e lies between -113 (2^15 for
 // the largest number) and 99 (2^-27 for the smallest normal one). The row pass's exponentials are 2^(s - m - e0), m
 // the running maximum of s + log2 f, e0 a group's -log2 f where its items share it, up to 28 (most exponentials are at
@@ -529,25 +532,13 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
       const int ll = ln & (32 * SG - 1);
       const int32_t lb = cs_lds<int32_t>(st + (ll >> 5) * 512 + CS_LAB * 128 + (ll & 31) * 4) >> 1;
       hit = __any((uint32_t)(lb - (int32_t)r0) < (uint32_t)(16 * UB));
-      // the label's element is to become |a| q (its sign follows in `patch`): fp32's scores are log2 p here;
-      // a bf16 score is the one whose exponential is |a| q, unless the row's weight is zero (ls infinite),
-      // which leaves nothing whatever the score
-      if (hit) {
+      // fp32: the label's element is to become |a| q (its sign follows in `patch`); the scores are log2 p here
+      if (NP == 2 && hit) {
         asm volatile("");  // keeps the rare path a branch
-        each_hit(
-            sg,
-            [&](int k) __attribute__((always_inline)) {
-              f32x4 x = cs_lds<f32x4>(stat_at(sg, CS_LQ, k));
-              if constexpr (NP == 1) {
-                const f32x4 ls = cs_lds<f32x4>(stat_at(sg, CS_LSE2, k));
-#pragma unroll
-                for (int r = 0; r < 4; ++r) x[r] = ls[r] == INFINITY ? 0.f : (x[r] + ls[r]) * (1.f / kw);
-              }
-              return x;
-            },
-            [&](int k, int ub, int r, bool is, float x) __attribute__((always_inline)) {
-              s.v[k][ub][r] = is ? x : s.v[k][ub][r];
-            });
+        each_hit(sg, [&](int k) __attribute__((always_inline)) { return cs_lds<f32x4>(stat_at(sg, CS_LQ, k)); },
+                 [&](int k, int ub, int r, bool is, float x) __attribute__((always_inline)) {
+                   s.v[k][ub][r] = is ? x : s.v[k][ub][r];
+                 });
       }
     } else {
       if constexpr (NP == 2) {
@@ -644,13 +635,33 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
       }
     }
   };
-  // the label's element of P is negative
-  auto patch = [&](uint32_t sg, Probs& pb) __attribute__((always_inline)) {
-    each_hit(sg, [](int) { return f32x4{}; }, [&](int k, int ub, int r, bool is, float) __attribute__((always_inline)) {
-      const uint32_t sign = is ? (r & 1 ? 0x80000000u : 0x8000u) : 0u;
+  // The label's element of P is negative. bf16: it is set here to |a| q rounded, and `rest` leaves what that rounding
+  // lost as a P of its own: the label's term is most of an item's gradient where it has one.
+  auto patch = [&](uint32_t sg, Probs& pb, bool rest) __attribute__((always_inline)) {
+    if constexpr (NP == 2) {
+      each_hit(sg, [](int) { return f32x4{}; }, [&](int k, int ub, int r, bool is, float) __attribute__((always_inline)) {
+        const uint32_t sign = is ? (r & 1 ? 0x80000000u : 0x8000u) : 0u;
 #pragma unroll
-      for (int pl = 0; pl < NP; ++pl) pb.w[k >> 1][ub][pl][2 * (k & 1) + (r >> 1)] ^= sign;
-    });
+        for (int pl = 0; pl < NP; ++pl) pb.w[k >> 1][ub][pl][2 * (k & 1) + (r >> 1)] ^= sign;
+      });
+    } else {
+      each_hit(sg,
+               [&](int k) __attribute__((always_inline)) {
+                 f32x4 v = cs_lds<f32x4>(stat_at(sg, CS_LQ, k));
+#pragma unroll
+                 for (int r = 0; r < 4; ++r) {
+                   const float q = __builtin_amdgcn_exp2f(v[r]), h = (float)(__bf16)q;
+                   v[r] = rest ? h - q : -h;
+                 }
+                 return v;
+               },
+               [&](int k, int ub, int r, bool is, float x) __attribute__((always_inline)) {
+                 const int i = 2 * (k & 1) + (r >> 1);
+                 const uint32_t keep = r & 1 ? 0xffffu : 0xffff0000u, bits = ib_pk(r & 1 ? 0.f : x, r & 1 ? x : 0.f);
+                 const uint32_t w = pb.w[k >> 1][ub][0][i];
+                 pb.w[k >> 1][ub][0][i] = is ? (w & keep) | (bits & ~keep) : w;
+               });
+    }
   };
   // rows of negative weight
   auto negate = [&](uint32_t sg, Probs& pb) __attribute__((always_inline)) {
@@ -731,11 +742,19 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
         if constexpr (MODE == CS_COL) {
           if (hit) {
             asm volatile("");  // keeps the rare path a branch
-            patch(sg, pb);
+            patch(sg, pb, false);
           }
           if (flip) negate(sg, pb);
         }
         if constexpr (MODE != CS_STATS) product(ln, bo, pb, al);
+        if constexpr (MODE == CS_COL && NP == 1)
+          if (hit) {
+            asm volatile("");  // keeps the rare path a branch
+            pb = Probs{};
+            patch(sg, pb, true);
+            if (flip) negate(sg, pb);
+            product(ln, bo, pb, al);
+          }
       }
     buf = buf + 1 == NB ? 0 : buf + 1;
   }

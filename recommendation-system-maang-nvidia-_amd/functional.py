@@ -1449,8 +1449,7 @@ def catalog_softmax_fwd(X, W, labels, scale: float = 1.0, weights=None, ignore_i
     A label outside [0, V) that is not ignore_index makes its row and the loss NaN. An item may be masked by a
     large negative or infinite logit (a bias column). Float32 operands keep about 22 bits under scales of their
     own for each row and item (include/recsys_hip.h has the bound), whatever a model's contraction_precision;
-    bfloat16 gradients come from probabilities rounded to bfloat16: their error against float64 is up to a third
-    more than the results' own rounding."""
+    in bfloat16 gradients the probabilities, but the label's own, are rounded to bfloat16."""
     return _catalog_fwd(X, W, labels, scale, weights, ignore_index, reduction, want_grad, True)
 
 

@@ -162,3 +162,21 @@ def test_an_only_item(cuda, dtype, N, D, scale, size):
     """The log sum of a catalogue of one item is its logit, to the roundings of the terms alone."""
     x, w, y, _ = inputs(N, 1, D, dtype, seed=N, ignored=0.5, scale=scale)
     check(x, (w.float() * size).to(dtype), y, None, scale)
+
+
+@pytest.mark.parametrize("N,V,D", [(500, 900, 128), (300, 70, 64), (700, 2000, 200)])
+@pytest.mark.parametrize("sign", [False, True])
+def test_label_terms_of_bf16_items_are_not_rounded(cuda, N, V, D, sign):
+    """Labels shared by many rows: an item's gradient is the difference of large label terms -a (1 - p_y) x, which
+    keep fp32's precision; half a step (2^-8) is for the result and for the other rows' p alone."""
+    x, w, y, _ = inputs(N, V, D, torch.bfloat16, seed=N)
+    y = y % 5
+    a = torch.linspace(-1.0, 1.5, N, device="cuda") if sign else None
+    r = reference(x, w, y, 1.0, a)
+    t = tolerances(r, N, V, D, torch.float32)
+    _, _, _, dw = step(x, w, y, a)
+    X, W, yc = x.double().cpu(), w.double().cpu(), y.cpu()
+    P = torch.softmax(X @ W.T, 1)
+    P[torch.arange(N), yc] = 0.0
+    P *= (a.double().cpu().abs() if sign else torch.ones(N, dtype=torch.float64))[:, None]
+    within(dw, r["dw"], t["dw"] + r["dw"].abs() * 2.0 ** -8 + 2.0 ** -8 * (P.T @ X.abs()), "dw")
