@@ -17,22 +17,24 @@
 // difference of nearly equal numbers where the label is nearly certain. The column pass takes -q for
 // the label's element.
 //
-// bf16 inputs: one bf16 product, p rounded to bf16 (2^-8 of each term, as its output is; a p in two terms would be
-// half as much matrix work again in each pass). The label's term keeps fp32's precision: dx has w_y itself, the column
-// pass a second product of what -q's rounding lost, in the groups of rows that hold a label of the wave's items
-// (16384 x 1M x 128: none in a thousand; 1021 x 50k x 96: 49 -> 54 us). fp32 inputs:
-// every operand as two fp16 terms h + l of the value scaled by a power of two (|x - h - l| <= 2^-22
-// |x|, or 2^-39 of the scale's largest value), three products h h, h l, l h per fp32 product: half the
-// matrix work of the exact three-term bf16 split. Every row of x and every item has a scale of its own, so
-// an item takes no bits from another. A logit's error is c sum_d |x_d w_d| 2^-20, like an fp32 product's own
-// rounding, plus c D 2^-30 max|x_n| max|w_v|: more than that only where an entry 2^10 and more below its item's
-// largest one meets an x that makes up for it. In both passes P carries the streamed row's scale and is itself scaled against a running maximum of
-// the scaled terms, so that unlikely or small items keep their relative precision, and each tile's sum is
-// formed in fresh accumulators and added in fp32 (the matrix unit's long running sums lose bits).
+// bf16 inputs: one bf16 product, p rounded to bf16 (2^-8 of each term, as its output is; p in two terms would
+// be half as much matrix work again in each pass). The label's term keeps fp32's precision: dx has w_y itself,
+// the column pass a second product of what -q's rounding lost, in the groups of rows that hold a label of the
+// wave's items (16384 x 1M x 128: one group in a thousand; 1021 x 50k x 96: 49 -> 54 us).
 //
-// Bound: the matrix cores' rate at the clock their load leaves (1.9 to 2.1 GHz; 54 to 63 % of the cycles
-// busy), the exponentials' vector work beside them. 16384 x 1M x 128 bf16, a training step: 13.4 to 14.0 ms,
-// 1.20 to 1.25 PFLOP/s of its 8 N V D flops (a large bf16 library product: 1.16); 8192 x 100k x 128 fp32:
+// fp32 inputs: every operand as two fp16 terms h + l of the value scaled by a power of two (|x - h - l| <=
+// 2^-22 |x|, or 2^-39 of the scale's largest value), three products h h, h l, l h per fp32 product: half the
+// matrix work of the exact three-term bf16 split. Every row of x and every item has a scale of its own, so an
+// item takes no bits from another. A logit's error is c sum_d |x_d w_d| 2^-20, like an fp32 product's own
+// rounding, plus c D 2^-30 max|x_n| max|w_v|: more than the former only where an entry 2^10 and more below its
+// item's largest one meets an x that makes up for it. In both passes P carries the streamed row's scale and is
+// itself scaled against a running maximum of the scaled terms, so that unlikely or small items keep their
+// relative precision, and each tile's sum is formed in fresh accumulators and added in fp32 (the matrix unit's
+// long running sums lose bits).
+//
+// Bound: the matrix cores' rate at the clock their load leaves (1.9 to 2.1 GHz; 52 to 68 % of the cycles
+// busy), the exponentials' vector work beside them. 16384 x 1M x 128 bf16, a training step: 13.1 to 14.2 ms,
+// 1.2 to 1.3 PFLOP/s of its 8 N V D flops (a large bf16 library product: 1.16); 8192 x 100k x 128 fp32:
 // 2.0 ms, 420 TFLOP/s, three fp16 products each (a large fp32 library product: 0.154 PFLOP/s). Fewer than ~300 rows:
 // the catalogue's bytes.
 #include "split.hpp"
