@@ -503,8 +503,8 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
   // Before a group's exponentials (its first streamed row is n0): the label's term leaves them and the
   // running maximum is raised (up, al: what that multiplies O and l by). Both are rare, and what they
   // change is small, so the common path has no branch between its matrix and vector instructions.
-  auto prepare = [&](int64_t n0, int ln, uint32_t st, uint32_t sg, Scores& s, float (&al)[UB], float (&kg)[UB], float& e0, bool& up,
-                     bool& hit) __attribute__((always_inline)) {
+  auto prepare = [&](int64_t n0, int ln, uint32_t st, uint32_t sg, Scores& s, float (&al)[UB], float (&kg)[UB],
+                     float& e0, bool& up, bool& hit) __attribute__((always_inline)) {
     up = hit = false;
     bool one = true;
     float ew = 0.f;  // -log2 f of the group's items, where they share it
@@ -680,8 +680,8 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
     }
   };
   // exponentials of part i = (subtile k, ub) of 2 SG UB
-  auto exponentials = [&](int i, uint32_t sg, const Scores& s, Probs& pb, const float (&kg)[UB], const float (&mg)[UB], float p0,
-                          float (&sum)[UB]) __attribute__((always_inline)) {
+  auto exponentials = [&](int i, uint32_t sg, const Scores& s, Probs& pb, const float (&kg)[UB], const float (&mg)[UB],
+                          float p0, float (&sum)[UB]) __attribute__((always_inline)) {
     const int k = i / UB, ub = i % UB;
     f32x4 ls, e, f = {};
     if constexpr (MODE == CS_COL && NP == 1) ls = cs_lds<f32x4>(stat_at(sg, CS_LSE2, k));
@@ -689,7 +689,8 @@ __global__ __launch_bounds__(64 * cs_cfg(D, NP, MODE).NW, cs_lb(D, NP, MODE)) vo
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const float x = s.v[k][ub][r];
-      if constexpr (MODE != CS_COL) e[r] = __builtin_amdgcn_exp2f(NP == 2 ? __builtin_fmaf(x, kg[ub], -mg[ub]) : __builtin_fmaf(x, kq[ub], -m[ub]));
+      if constexpr (MODE != CS_COL)
+        e[r] = __builtin_amdgcn_exp2f(NP == 2 ? __builtin_fmaf(x, kg[ub], -mg[ub]) : __builtin_fmaf(x, kq[ub], -m[ub]));
       else if constexpr (NP == 2) e[r] = __builtin_amdgcn_exp2f(x - m[ub]);
       else e[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x, kw, -ls[r]));
     }
@@ -957,8 +958,8 @@ struct CsImage {
 };
 
 // x [N, D] and w [V, D] into padded 16-bit rows: two fp16 planes of the scaled values (fp32), with w's
-// statistics (up to a whole tile), or a copy (bf16). A row of x whose label is the ignored one keeps its finite entries only (its weight in the
-// column pass is zero, and zero times infinity would not be). 4 columns per lane.
+// statistics (up to a whole tile), or a copy (bf16). A row of x that takes no part keeps its finite entries only
+// (its weight in the column pass is zero, and zero times infinity would not be). 4 columns per lane.
 template <int DP, int NP>
 __global__ __launch_bounds__(256) void cs_image_kernel(CsImage p) {
   constexpr int LPR = DP / 4, RPB = 256 / LPR;  // lanes per row, rows per workgroup
